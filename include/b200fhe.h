@@ -330,6 +330,38 @@ int b2_ct_lincomb(b2_ctx *ctx, size_t size_Ql, size_t n_poly, size_t n_terms, co
 int b2_poly_scalar(b2_ctx *ctx, int op, size_t n_limbs, const uint64_t *d_a, const uint64_t *h_scalars,
                    uint64_t *d_out, void *stream);
 
+/* Operators of generation with an encrypted model, next to its attention products (src/attention.cu:10-98); no counterpart in
+ * the reference, whose K/V ciphertexts are lists that its application keeps in Python.
+ *
+ * b2_pages_move: pages of a cache of two-polynomial ciphertexts, d_pool [planes][pages][2][limbs][N]. In every plane, page dst[i]
+ * becomes what page src[i] was before the call, for all i at once: copies, one page into many, permutations in place. src[i] < 0:
+ * a page of zeros. d_src null (or d_pool): the pool itself; else another one, [planes][src_pages][2][src_limbs][N] with
+ * src_limbs >= limbs, of which the first `limbs` limbs of each polynomial are taken (mod_switch_to). dst and src are HOST arrays
+ * of n, read at the call; destinations are distinct. No scratch; each thread owns the same 32 bytes of every page. */
+int b2_pages_move(b2_ctx *ctx, size_t limbs, size_t planes, uint64_t *d_pool, size_t pages, const uint64_t *d_src,
+                  size_t src_limbs, size_t src_pages, size_t n, const int64_t *dst, const int64_t *src, void *stream);
+/* b2_multiply_sum: for every query g, the three polynomials of sum_t a[g * terms + t] x b[t] (b2_tensor_mul, summed), so that one
+ * relinearisation serves all terms. Operands are two-polynomial ciphertexts of la and lb limbs a polynomial, of which the first
+ * size_Ql count; d_a [queries * terms] and d_b [terms] are HOST arrays of device pointers. d_out [queries][3][size_Ql][N], apart
+ * from the operands. */
+int b2_multiply_sum(b2_ctx *ctx, size_t size_Ql, size_t queries, size_t terms, const uint64_t *const *d_a, size_t a_limbs,
+                    const uint64_t *const *d_b, size_t b_limbs, uint64_t *d_out, void *stream);
+/* b2_rotary_factors: the slot values by which a ciphertext of `per` = slots / (heads * d_head) positions is rotated, for `tokens`
+ * positions in ceil(tokens / per) ciphertexts: theta[t][j] = position[t][axis[j]] * inv_freq[j] (rounded to a double), slot
+ * (t mod per) * heads * d_head + h * d_head + i of ciphertext t / per.
+ *   packing 0 (a slot holds x + i y of a pair; slot i = pair i): d_out [1][ciphertexts][slots] = scaling * exp(i theta), 1 where
+ *             i >= pairs;
+ *   packing 1 (real slots, pair j = slots j and j + pairs), 2 (pair j = slots 2 j and 2 j + 1): d_out [3][ciphertexts][slots] =
+ *             C, A, B of  x C + rot(x, s) A + rot(x, -s) B, s = pairs or 1: scaling * cos in C, -sin in A at a pair's first slot,
+ *             sin in B at its second; C = 1 where a head has no pair;
+ *   conjugate != 0: the inverse rotation. A token with keep == 0 (d_keep may be null), and slots of no token: zeros.
+ * Positions [token][axis] of type pos_type (0 int32, 1 int64, 2 float, 3 double) with strides in elements; d_axis int32 [pairs],
+ * d_keep bytes with a stride; d_out complex doubles. tokens = 0 writes nothing. */
+int b2_rotary_factors(b2_ctx *ctx, int packing, size_t tokens, size_t heads, size_t d_head, size_t pairs,
+                      const void *d_positions, int pos_type, int64_t pos_stride, int64_t axis_stride,
+                      const double *d_inv_freq, const int32_t *d_axis, const uint8_t *d_keep, int64_t keep_stride,
+                      double scaling, int conjugate, void *d_out, void *stream);
+
 /* RNS-limb sharding of one key switch over `world` GPUs (no counterpart in the reference, which
  * has no multi-GPU path; replaces keyswitch_inplace, src/eval_key_switch.cu:294-381, on a slice).
  * Rank r owns the Q limbs [r l/world, (r+1) l/world) and the P limbs [r alpha/world, (r+1) alpha/world).

@@ -5,7 +5,7 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRCS = [os.path.join(HERE, "csrc", f) for f in ("b200fhe.cu", "ntt_whole.cu")]  # compiled side by side
+SRCS = [os.path.join(HERE, "csrc", f) for f in ("b200fhe.cu", "ntt_whole.cu", "cache.cu")]  # compiled side by side
 OUT = os.path.join(HERE, "libb200fhe.so")
 DEPS = glob.glob(os.path.join(HERE, "csrc", "*")) + [os.path.join(os.path.dirname(HERE), "include", "b200fhe.h")]
 FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-Xcompiler", "-fPIC,-fopenmp"]

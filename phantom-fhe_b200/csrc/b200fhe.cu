@@ -13,6 +13,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -24,6 +25,7 @@
 #include "elementwise.cuh"
 #include "launch.cuh"
 #include "ntt_whole.cuh"
+#include "cache.cuh"
 
 using namespace b2;
 typedef unsigned __int128 u128_t;
@@ -2612,6 +2614,107 @@ extern "C" int b2_ct_lincomb(b2_ctx *c, size_t l, size_t n_poly, size_t n_terms,
     launch_k(lincomb_kernel, dim3((unsigned)(c->N / 256), (unsigned)(n_poly * l)), 256, 0, (cudaStream_t)stream, a, d_out, c->d_mod, (uint32_t)c->N, (uint32_t)l,
              (uint32_t)n_terms, n_poly > 3 ? 2u : (uint32_t)n_poly);
     LAUNCH_CHECK("lincomb_kernel");
+    return B2_OK;
+}
+
+// ------------------------------------------------------------------------------------------------
+// operators of generation with an encrypted model (cache.cuh)
+// ------------------------------------------------------------------------------------------------
+// How many lanes (blockIdx.y) a launch of page moves is spread over: enough that the grid fills the GPU's resident threads
+static uint32_t page_lanes(const b2_ctx *c, size_t limbs, size_t planes, size_t parts) {
+    const size_t ctas = limbs * c->N / 512 * planes, want = (size_t)c->sm_count * 8;  // of 256 threads with 32 bytes a page each
+    return (uint32_t)std::max<size_t>(1, std::min({(want + ctas - 1) / ctas, parts, (size_t)PAGE_LANES}));
+}
+
+extern "C" int b2_pages_move(b2_ctx *c, size_t limbs, size_t planes, uint64_t *d_pool, size_t pages, const uint64_t *d_src, size_t src_limbs,
+                             size_t src_pages, size_t n, const int64_t *dst, const int64_t *src, void *stream) {
+    CHECK_CTX(c);
+    CHECK_LEVEL(c, limbs);
+    const bool apart = d_src && d_src != d_pool;
+    if (!apart) d_src = d_pool, src_limbs = limbs, src_pages = pages;
+    if (!d_pool || (n && (!dst || !src))) return fail(B2_EINVAL, "pages_move: null pointer");
+    if (planes < 1 || planes > 65535 || pages < 1 || pages > PAGE_MAX || src_pages < 1 || src_pages > PAGE_MAX)
+        return fail(B2_EINVAL, "pages_move: 1 to 65535 planes and at least one page are wanted");
+    if (src_limbs < limbs || src_limbs > c->size_Q) return fail(B2_EINVAL, "pages_move: the source must be at the pool's level or above it");
+    if (!aligned32(d_pool) || !aligned32(d_src)) return fail(B2_EINVAL, "device buffers must be 32-byte aligned (256-bit accesses)");
+    for (size_t i = 0; i < n; i++) {
+        if (dst[i] < 0 || (uint64_t)dst[i] >= pages) return fail(B2_EINVAL, "pages_move: destination page out of range");
+        if (src[i] >= 0 && (uint64_t)src[i] >= src_pages) return fail(B2_EINVAL, "pages_move: source page out of range");
+    }
+    PageArgs a{};
+    a.pool = d_pool, a.src = d_src;
+    a.half = (uint32_t)(limbs * c->N), a.src_gap = (uint32_t)((src_limbs - limbs) * c->N);
+    a.page = 2 * (uint64_t)limbs * c->N, a.src_page = 2 * (uint64_t)src_limbs * c->N;
+    a.plane = a.page * pages, a.src_plane = a.src_page * src_pages;
+    if (apart && (uintptr_t)d_src < (uintptr_t)(d_pool + a.plane * planes) && (uintptr_t)d_pool < (uintptr_t)(d_src + a.src_plane * planes))
+        return fail(B2_EINVAL, "pages_move: the source overlaps the pool without being it");
+    try {
+        std::vector<int64_t> seen(dst, dst + n);
+        std::sort(seen.begin(), seen.end());
+        if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) return fail(B2_EINVAL, "pages_move: a destination page is named twice");
+        std::vector<uint32_t> first;
+        const PagePlan plan = plan_pages(n, dst, src, apart, PAGE_STEPS, first);
+        pack_pages(
+            plan, first, PAGE_STEPS, [&](size_t parts) { return page_lanes(c, limbs, planes, parts); },
+            [&](uint32_t begin, const std::vector<uint32_t> &ends) {
+                LaunchScope ls(c, (cudaStream_t)stream, "pages_move");
+                launch_pages_move(a, plan.steps.data() + begin, ends.data(), (uint32_t)ends.size(), (uint32_t)planes, (cudaStream_t)stream);
+            });
+    } catch (const std::bad_alloc &) {
+        return fail(B2_ENOMEM, "pages_move: out of host memory");
+    }
+    LAUNCH_CHECK("pages_move_kernel");
+    return B2_OK;
+}
+
+extern "C" int b2_multiply_sum(b2_ctx *c, size_t l, size_t queries, size_t terms, const uint64_t *const *d_a, size_t la, const uint64_t *const *d_b,
+                               size_t lb, uint64_t *d_out, void *stream) {
+    CHECK_CTX(c);
+    CHECK_LEVEL(c, l);
+    if (!d_a || !d_b || !d_out || queries < 1 || terms < 1) return fail(B2_EINVAL, "multiply_sum: bad argument (one query and one term at least)");
+    if (la < l || lb < l || la > c->size_Q || lb > c->size_Q) return fail(B2_EINVAL, "multiply_sum: an operand is below the level");
+    bool ok = aligned32(d_out);
+    for (size_t i = 0; i < queries * terms; i++) ok = ok && d_a[i] && aligned32(d_a[i]);
+    for (size_t i = 0; i < terms; i++) ok = ok && d_b[i] && aligned32(d_b[i]);
+    if (!ok) return fail(B2_EINVAL, "multiply_sum: operands must be there and 32-byte aligned");
+    for (size_t q0 = 0; q0 < queries; q0 += SUM_QUERIES) {
+        const size_t g = std::min<size_t>(SUM_QUERIES, queries - q0);
+        for (size_t t0 = 0; t0 < terms; t0 += SUM_TERMS) {
+            const size_t n = std::min<size_t>(SUM_TERMS, terms - t0);
+            SumArgs a{};
+            a.out = d_out + q0 * 3 * l * c->N, a.mod = c->d_mod, a.logN = (uint32_t)c->logN;
+            a.l = (uint32_t)l, a.la = (uint32_t)la, a.lb = (uint32_t)lb, a.terms = (uint32_t)n, a.first = t0 == 0;
+            std::copy_n(d_b + t0, n, a.b);
+            for (size_t q = 0; q < g; q++) std::copy_n(d_a + (q0 + q) * terms + t0, n, a.a + q * n);
+            LaunchScope ls(c, (cudaStream_t)stream, "multiply_sum");
+            launch_multiply_sum(a, (uint32_t)g, (cudaStream_t)stream);
+        }
+    }
+    LAUNCH_CHECK("multiply_sum_kernel");
+    return B2_OK;
+}
+
+extern "C" int b2_rotary_factors(b2_ctx *c, int packing, size_t tokens, size_t heads, size_t d_head, size_t pairs, const void *d_pos, int pos_type,
+                                 int64_t pos_stride, int64_t axis_stride, const double *d_inv_freq, const int32_t *d_axis, const uint8_t *d_keep,
+                                 int64_t keep_stride, double scaling, int conjugate, void *d_out, void *stream) {
+    CHECK_CTX(c);
+    if (packing < ROTARY_PAIRS || packing > ROTARY_INTERLEAVED || pos_type < 0 || pos_type > 3) return fail(B2_EINVAL, "rotary_factors: unknown packing or position type");
+    const size_t slots = c->N / 2;
+    if (heads < 1 || d_head < 1 || heads > slots || d_head > slots || heads * d_head > slots) return fail(B2_EINVAL, "rotary_factors: heads * d_head must be in [1, slots]");
+    if (pairs < 1 || pairs > (packing == ROTARY_PAIRS ? d_head : d_head / 2)) return fail(B2_EINVAL, "rotary_factors: more pairs than a head holds");
+    if (tokens == 0) return B2_OK;
+    if (!d_pos || !d_inv_freq || !d_axis || !d_out) return fail(B2_EINVAL, "rotary_factors: null pointer");
+    if ((uintptr_t)d_out & 15) return fail(B2_EINVAL, "rotary_factors: the result must be 16-byte aligned");
+    const size_t per = slots / (heads * d_head);
+    if (tokens > 0x40000000) return fail(B2_ESIZE, "rotary_factors: more than 2^30 positions in one call");
+    RotaryArgs a{};
+    a.out = (double2 *)d_out, a.pos = d_pos, a.inv_freq = d_inv_freq, a.axis = d_axis, a.keep = d_keep;
+    a.pos_t = pos_stride, a.pos_a = axis_stride, a.keep_t = keep_stride, a.scaling = scaling, a.conjugate = conjugate ? 1u : 0u;
+    a.tokens = (uint32_t)tokens, a.heads = (uint32_t)heads, a.d_head = (uint32_t)d_head, a.pairs = (uint32_t)pairs;
+    a.per = (uint32_t)per, a.slots = (uint32_t)slots, a.cts = (uint32_t)((tokens + per - 1) / per);
+    LaunchScope ls(c, (cudaStream_t)stream, "rotary_factors");
+    launch_rotary_factors(a, packing, pos_type, c->sm_count, (cudaStream_t)stream);
+    LAUNCH_CHECK("rotary_factors_kernel");
     return B2_OK;
 }
 

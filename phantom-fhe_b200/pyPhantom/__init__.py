@@ -570,6 +570,52 @@ def multiply(ctx, a, b):
     return a._like(out, scale=a._scale * b._scale)
 
 
+def multiply_sum(ctx, a, b):
+    """sum_t a[t] x b[t] of two lists of two-polynomial ciphertexts, as one three-polynomial ciphertext at the lower of the two
+    lists' levels: the tensor products of `multiply`, summed in one launch, so that one `relinearize` (and one rescale) serves all
+    of them. Where a is a list of lists (several weightings of the same b), each gives a result and b is read for up to four of them
+    at a time. No counterpart in the reference, which relinearises every product (src/attention.cu:60-90)."""
+    if not len(b):
+        raise ValueError("encrypteds cannot be empty")
+    first = _same_kind(ctx, b)
+    data = [ct.data.contiguous() for ct in b]
+    return _multiply_sum(ctx, a, np.array([t.data_ptr() for t in data], dtype=np.uint64), first._limbs, first._chain_index, first._scale)
+
+
+def _same_kind(ctx, cts):
+    first = cts[0]
+    for ct in cts:
+        if ct._chain_index != first._chain_index or ct._limbs != first._limbs or ct._N != ctx.N:
+            raise ValueError("encrypted1 and encrypted2 parameter mismatch")
+        if not ct._is_ntt_form:
+            raise ValueError("encrypted1 and encrypted2 must be in NTT form")
+        if ct._size != 2:
+            raise ValueError("only 2-polynomial operands are built")
+        if ct._scale != first._scale and not _are_close(ct._scale, first._scale):
+            raise ValueError("scale mismatch")
+    return first
+
+
+def _multiply_sum(ctx, a, table, b_limbs, b_chain_index, b_scale):
+    """a: a list of ciphertexts or a list of such lists; table: the addresses of the other operands"""
+    if not len(a):
+        raise ValueError("encrypteds cannot be empty")
+    many = isinstance(a[0], (list, tuple))
+    rows = a if many else [a]
+    if any(len(r) != len(table) for r in rows) or not len(table):
+        raise ValueError("multiply_sum: as many ciphertexts in every list are wanted, and at least one")
+    cts = [ct for r in rows for ct in r]
+    first = _same_kind(ctx, cts)
+    held = [ct.data.contiguous() for ct in cts]  # strided views become copies, which live until the launch
+    tab = np.array([t.data_ptr() for t in held], dtype=np.uint64)
+    l = min(first._limbs, b_limbs)
+    out = ctx.empty(len(rows), 3, l)
+    with _native.on_device(ctx):
+        check(LIB.b2_multiply_sum(ctx._h, l, len(rows), len(table), tab.ctypes.data, first._limbs, table.ctypes.data, b_limbs, out.data_ptr(), _stream()))
+    res = [first._like(out[g], chain_index=max(first._chain_index, b_chain_index), scale=first._scale * b_scale) for g in range(len(rows))]
+    return res if many else res[0]
+
+
 def _key_table(ctx, key, l):
     if key.dnum() < ctx.beta(l):
         raise ValueError("key has fewer digits than this level needs")
@@ -657,6 +703,18 @@ def rescale_to_next(ctx, ct):
     out = ctx.empty(ct._size, l - 1)
     ws, nbytes = ctx.workspace(_native.OP_RESCALE, l)
     check(LIB.b2_rescale(ctx._h, l, ct._size, ct.data.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes, _stream()))
+    return ct._like(out, chain_index=ct._chain_index + 1, scale=ct._scale / float(ctx.primes[l - 1]))
+
+
+def _rescale_rounded(ctx, ct):
+    """rescale_to_next that rounds to nearest (b2_rescale_rounded): without the half unit of every coefficient that flooring leaves,
+    which adds up in the slots whose root is near 1"""
+    if ct._chain_index == ctx.size_Q:
+        raise ValueError("end of modulus switching chain reached")
+    l = ct._limbs
+    out = ctx.empty(ct._size, l - 1)
+    ws, nbytes = ctx.workspace(_native.OP_RESCALE, l)
+    check(LIB.b2_rescale_rounded(ctx._h, l, ct._size, ct.data.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes, _stream()))
     return ct._like(out, chain_index=ct._chain_index + 1, scale=ct._scale / float(ctx.primes[l - 1]))
 
 
@@ -1214,3 +1272,5 @@ from .blocks import eval_polynomial, inner_sum, replicate  # noqa: E402,F401
 from .model_blocks import (compute_qkt, finalize_softmax, mlp_forward, mlp_forward_complex, mlp_weights,  # noqa: E402,F401
                            mlp_weights_complex, ps_exp_init, rmsnorm_forward, rmsnorm_params, rmsnorm_weights,
                            score_times_v, softmax_correct, square_iterations_damped_inplace, square_iterations_inplace)
+from .cache import cached_qkt, cached_score_times_v, ciphertext_cache  # noqa: E402,F401
+from .rotary import rotary  # noqa: E402,F401

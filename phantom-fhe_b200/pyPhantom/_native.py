@@ -3,6 +3,7 @@
 There is no CPU fallback: if the shared library is missing or has no CUDA device to run on,
 importing or creating a context raises.
 """
+import contextlib
 import ctypes
 import os
 
@@ -11,7 +12,7 @@ import torch
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG, "libb200fhe.so")
 
-_sz, _u64, _vp, _int, _u32 = ctypes.c_size_t, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32
+_sz, _u64, _i64, _vp, _int, _u32 = ctypes.c_size_t, ctypes.c_uint64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32
 
 # name -> (restype, argtypes); mirrors include/b200fhe.h declaration by declaration
 SIGNATURES = {
@@ -79,6 +80,9 @@ SIGNATURES = {
     "b2_ct_scalar": (_int, [_vp, _sz, _sz, _vp, _vp, _vp, _vp]),
     "b2_ct_lincomb": (_int, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b2_poly_scalar": (_int, [_vp, _int, _sz, _vp, _vp, _vp, _vp]),
+    "b2_pages_move": (_int, [_vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _vp, _vp]),
+    "b2_multiply_sum": (_int, [_vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp]),
+    "b2_rotary_factors": (_int, [_vp, _int, _sz, _sz, _sz, _sz, _vp, _int, _i64, _i64, _vp, _vp, _vp, _i64, ctypes.c_double, _int, _vp, _vp]),
     "b2_ctx_set_shard": (_int, [_vp, _int, _int]),
     "b2_shard_limbs": (_int, [_vp, _sz, _vp]),
     "b2_shard_keyswitch_phase": (_int, [_vp, _sz, _int, _vp, _vp, _sz, _vp, _vp, _sz, _vp]),
@@ -129,3 +133,11 @@ def _stream_lookup():
 
 
 current_stream = _stream_lookup()
+
+
+_NOTHING = contextlib.nullcontext()
+
+
+def on_device(ctx):
+    """a context manager that makes the context's device the current one, so that current_stream() is a stream of it"""
+    return _NOTHING if torch.cuda.current_device() == ctx.device else torch.cuda.device(ctx.device)

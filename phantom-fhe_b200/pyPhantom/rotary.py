@@ -1,0 +1,133 @@
+"""Rotary positions on encrypted queries and keys (no counterpart in the reference: its application rotates before it encrypts).
+
+Position p turns pair j of every head by theta_j = p[axis[j]] * inv_freq[j]; with several axes (time, height, width of a video's
+patches) each pair follows one of them. Heads lie in the slots as compute_qkt reads them (src/attention.cu:10-28): slot
+t * heads * d_head + h * d_head + i of a ciphertext holds element i of head h at its t-th position.
+
+  packing "pairs"        a slot holds x + i y of a pair (what matrices folded into complex ones deliver): one product with
+                         exp(i theta), no key switch. q . k is then the real part of the sum over q' conj(k'): conjugate k' once
+                         (`rotate(ct, 0)`) as it goes into the cache.
+  packing "halves"       real slots, pair j = elements j and j + pairs; x C + rot(x, s) A + rot(x, -s) B with s = pairs
+  packing "interleaved"  the same with pair j = elements 2 j and 2 j + 1, s = 1: two rotations from one decomposition
+
+Elements of a head beyond its pairs pass unchanged. Positions that are dropped (`keep`), and slots of no position, come out as zeros:
+a decoding step's one position goes into its place of a page that way, without a mask of its own.
+"""
+import torch
+
+from . import _rescale_rounded, add, hoist_rotations, multiply_plain, plaintext
+from ._native import LIB, check, current_stream as _stream, on_device
+
+_PACKINGS = {"pairs": 0, "halves": 1, "interleaved": 2}
+_POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
+CHUNK = 16  # ciphertexts whose factors are encoded at a time
+
+
+class rotary:
+    def __init__(self, context, inv_freq, heads, d_head, axes=None, packing="pairs", scaling=1.0):
+        """inv_freq: the angle per position of each pair (a sequence or a tensor); axes: the axis of each pair, 0 if not given;
+        scaling: a factor on sines and cosines"""
+        if packing not in _PACKINGS:
+            raise ValueError("rotary: packing is 'pairs', 'halves' or 'interleaved'")
+        f = torch.as_tensor(inv_freq, dtype=torch.float64).reshape(-1).to(device=context.device).contiguous()
+        heads, d_head, pairs = int(heads), int(d_head), f.numel()
+        if heads < 1 or d_head < 1 or heads * d_head > context.N // 2:
+            raise ValueError("rotary: heads * d_head must be in [1, slots]")
+        if pairs < 1 or pairs > (d_head if packing == "pairs" else d_head // 2):
+            raise ValueError("rotary: more pairs than a head holds")
+        a = [0] * pairs if axes is None else [int(v) for v in axes]
+        if len(a) != pairs or min(a) < 0:
+            raise ValueError("rotary: an axis for every pair is wanted")
+        self.ctx, self.heads, self.d_head, self.pairs, self.packing, self.scaling = context, heads, d_head, pairs, packing, float(scaling)
+        self.n_axes = max(a) + 1
+        self.positions_per_ct = context.N // 2 // (heads * d_head)
+        self.inv_freq, self.axes = f, torch.tensor(a, dtype=torch.int32, device=context.device)
+        self.step = pairs if packing == "halves" else 1
+
+    def factors(self, positions, keep=None, conjugate=False):
+        """The factors of `positions` ([tokens] or [tokens][axes], int32, int64, float32 or float64, any strides) as complex128
+        [vectors][ciphertexts][slots], one vector ("pairs") or three (C, A, B), positions_per_ct tokens to a ciphertext. keep: bool
+        [tokens], False for a token whose slots become zeros. conjugate: the inverse rotation."""
+        ctx, p = self.ctx, positions
+        if p.dim() == 1:
+            p = p.unsqueeze(1)
+        if p.dim() != 2 or p.dtype not in _POSITIONS:
+            raise ValueError("rotary: positions are [tokens] or [tokens][axes] of int32, int64, float32 or float64")
+        if p.shape[1] < self.n_axes:
+            raise ValueError("rotary: positions have fewer axes than the pairs name")
+        if keep is not None and (keep.dtype != torch.bool or keep.dim() != 1 or keep.shape[0] != p.shape[0]):
+            raise ValueError("rotary: keep is one truth value a token")
+        if p.get_device() != ctx.device or (keep is not None and keep.get_device() != ctx.device):
+            raise ValueError("rotary: positions and keep must lie on the context's device")
+        tokens = p.shape[0]
+        out = torch.empty(1 if self.packing == "pairs" else 3, -(-tokens // self.positions_per_ct), ctx.N // 2, dtype=torch.complex128, device=ctx.device)
+        with on_device(ctx):
+            check(LIB.b2_rotary_factors(ctx._h, _PACKINGS[self.packing], tokens, self.heads, self.d_head, self.pairs, p.data_ptr(), _POSITIONS[p.dtype],
+                                        p.stride(0), p.stride(1), self.inv_freq.data_ptr(), self.axes.data_ptr(), 0 if keep is None else keep.data_ptr(),
+                                        0 if keep is None else keep.stride(0), self.scaling, int(bool(conjugate)), out.data_ptr(), _stream()))
+        return out
+
+    def encode(self, encoder, factors, chain_index):
+        """[vector][ciphertext] plaintexts of `factors` at a level, at the scale of the prime that the rescale after the product
+        removes. Queries and keys of all layers at that level and of these positions share them."""
+        ctx = self.ctx
+        if factors.dim() != 3 or factors.dtype != torch.complex128 or factors.shape[2] != ctx.N // 2:
+            raise ValueError("rotary: factors are complex128 [vectors][ciphertexts][slots]")
+        if chain_index < 1:
+            raise ValueError("chain index out of range")
+        l = ctx.limbs_at(chain_index)
+        if l < 2:
+            raise ValueError("end of modulus switching chain reached")
+        scale = float(ctx.primes[l - 1])
+        if scale * max(1.0, abs(self.scaling)) * 1.4143 >= 2.0 ** 61:  # no coefficient exceeds it, and none may pass 62 bits
+            raise ValueError("scale out of bounds")
+        vecs, n = factors.shape[0], factors.shape[1]
+        if n == 0:
+            return [[] for _ in range(vecs)]
+        vals = factors.to(device=ctx.device).clone(memory_format=torch.contiguous_format)  # overwritten by the transform
+        coeffs, data = torch.empty(vecs * n, ctx.N, dtype=torch.int64, device=ctx.device), ctx.empty(vecs, n, l)
+        with on_device(ctx):
+            for k, z in enumerate(vals.view(vecs * n, -1)):
+                check(LIB.b2_encode_coeffs(ctx._h, z.data_ptr(), encoder._d_rot.data_ptr(), encoder._d_ksi.data_ptr(), scale / encoder.slots,
+                                           coeffs[k].data_ptr(), _stream()))
+            check(LIB.b2_expand_single_chain_batch(ctx._h, l, vecs * n, coeffs.data_ptr(), data.data_ptr(), _stream()))
+        return [[self._plain(data[v, i], chain_index, l, scale) for i in range(n)] for v in range(vecs)]
+
+    def _plain(self, data, chain_index, l, scale):
+        pt = plaintext()
+        pt._chain_index, pt._N, pt._limbs, pt._scale, pt.data = chain_index, self.ctx.N, l, scale, data
+        return pt
+
+    def apply(self, xs, plaintexts, galois_key=None):
+        """the ciphertexts xs rotated by the encoded factors, one level further down (rounded to nearest), at their scale. "halves" and "interleaved"
+        want a Galois key for the steps +-`step`."""
+        ctx = self.ctx
+        vecs = 1 if self.packing == "pairs" else 3
+        if len(plaintexts) != vecs or any(len(v) != len(xs) for v in plaintexts):
+            raise ValueError("rotary: as many encoded factors as ciphertexts are wanted")
+        if vecs == 3 and xs and galois_key is None:
+            raise ValueError("Galois key not present")
+        out = []
+        with on_device(ctx):
+            for i, x in enumerate(xs):
+                y = multiply_plain(ctx, x, plaintexts[0][i])
+                if vecs == 3:
+                    up, down = hoist_rotations(ctx, x, galois_key, [self.step, -self.step])
+                    y = add(ctx, add(ctx, y, multiply_plain(ctx, up, plaintexts[1][i])), multiply_plain(ctx, down, plaintexts[2][i]))
+                y = _rescale_rounded(ctx, y)
+                y.set_scale(x._scale)
+                out.append(y)
+        return out
+
+    def forward(self, encoder, xs, positions, keep=None, conjugate=False, galois_key=None):
+        """factors, encode and apply for ciphertexts of one level, CHUNK of them at a time"""
+        f = self.factors(positions, keep, conjugate)
+        if f.shape[1] != len(xs):
+            raise ValueError("rotary: positions for ceil(tokens / positions_per_ct) ciphertexts were given")
+        out = []
+        for i in range(0, len(xs), CHUNK):
+            part = xs[i:i + CHUNK]
+            if any(x._chain_index != part[0]._chain_index for x in part):
+                raise ValueError("encrypted and plain parameter mismatch")
+            out += self.apply(part, self.encode(encoder, f[:, i:i + CHUNK], part[0]._chain_index), galois_key)
+        return out
