@@ -3,62 +3,53 @@
 #include "launch.cuh"
 #include "sums.cuh"
 
+#include <type_traits>
+
 namespace b2 {
 
 // ---- pages ------------------------------------------------------------------------------------------------------------
 // A thread owns the same 32 bytes of every page and walks its lane's steps, so that moves of a pool onto itself need no second
 // buffer and no order between threads. Loads of a batch of steps go out before its stores: no step reads what an earlier step of
 // the plan wrote, whichever is issued first. Steps of one source that follow one another read it once.
+// Bound by HBM: a copy's rate, half reads and half writes. Four steps a batch keep the registers at 64, so that an SM has 1024
+// threads with 128 bytes each in flight; with eight (126 registers, 512 threads) 47 pages of 2 MB in four planes change places in
+// 159 us, with four in 124 (6.36 TB/s), with two in 130.
 template <int CAP>
 struct PageMoves {
     PageArgs a;
     uint16_t end[PAGE_LANES];
     PageStep step[CAP];
 };
+constexpr int PAGE_BATCH = 4;
 
-template <int COLS, int STEPS, int CAP>
-__global__ void __launch_bounds__(256) pages_move_kernel(const __grid_constant__ PageMoves<CAP> m) {
+template <int CAP>
+__global__ void __launch_bounds__(256, 4) pages_move_kernel(const __grid_constant__ PageMoves<CAP> m) {
     pdl_enter();
     const PageArgs &a = m.a;
-    const uint32_t lane = blockIdx.y, c0 = (blockIdx.x * 256 * COLS + threadIdx.x) * 4;
+    const uint32_t lane = blockIdx.y, c0 = (blockIdx.x * 256 + threadIdx.x) * 4;
     uint64_t *const pool = a.pool + (size_t)blockIdx.z * a.plane + c0;
-    const uint64_t *src[COLS];
-#pragma unroll
-    for (int j = 0; j < COLS; j++)
-        src[j] = a.src + (size_t)blockIdx.z * a.src_plane + c0 + j * 1024 + (c0 + j * 1024 >= a.half ? a.src_gap : 0);
-    u64x4 kept[COLS];
+    const uint64_t *const src = a.src + (size_t)blockIdx.z * a.src_plane + c0 + (c0 >= a.half ? a.src_gap : 0);
+    u64x4 kept = {0, 0, 0, 0};
     const uint32_t end = m.end[lane];
-    for (uint32_t k = lane ? m.end[lane - 1] : 0; k < end; k += STEPS) {
-        u64x4 v[STEPS][COLS];
-        uint32_t from[STEPS];
+    for (uint32_t k = lane ? m.end[lane - 1] : 0; k < end; k += PAGE_BATCH) {
+        u64x4 v[PAGE_BATCH];
+        uint32_t from[PAGE_BATCH];
 #pragma unroll
-        for (int u = 0; u < STEPS; u++) from[u] = k + u < end ? m.step[k + u].src : PAGE_KEPT;
-#pragma unroll
-        for (int u = 0; u < STEPS; u++) {
-            const uint32_t s = from[u];
-            if (u && s == from[u ? u - 1 : 0]) {
-#pragma unroll
-                for (int j = 0; j < COLS; j++) v[u][j] = v[u - 1][j];
-            } else if (s < PAGE_KEPT) {
-#pragma unroll
-                for (int j = 0; j < COLS; j++) v[u][j] = ld256(src[j] + (size_t)s * a.src_page);
-            } else {
-#pragma unroll
-                for (int j = 0; j < COLS; j++) v[u][j] = u64x4{0, 0, 0, 0};
-            }
+        for (int u = 0; u < PAGE_BATCH; u++) {
+            const uint32_t s = from[u] = k + u < end ? m.step[k + u].src : PAGE_KEPT;
+            if (u && s == from[u ? u - 1 : 0]) v[u] = v[u ? u - 1 : 0];
+            else if (s < PAGE_KEPT) v[u] = ld256(src + (size_t)s * a.src_page);
+            else v[u] = u64x4{0, 0, 0, 0};
         }
 #pragma unroll
-        for (int u = 0; u < STEPS; u++) {
+        for (int u = 0; u < PAGE_BATCH; u++) {
             if (k + u < end) {
                 const uint32_t to = m.step[k + u].dst;
-#pragma unroll
-                for (int j = 0; j < COLS; j++) {
-                    if (to == PAGE_KEPT) {
-                        kept[j] = v[u][j];
-                    } else {
-                        const u64x4 x = from[u] == PAGE_KEPT ? kept[j] : v[u][j];
-                        st256(pool + (size_t)to * a.page + j * 1024, x.a, x.b, x.c, x.d);
-                    }
+                if (to == PAGE_KEPT) {
+                    kept = v[u];
+                } else {
+                    const u64x4 x = from[u] == PAGE_KEPT ? kept : v[u];
+                    st256(pool + (size_t)to * a.page, x.a, x.b, x.c, x.d);
                 }
             }
         }
@@ -69,17 +60,10 @@ template <int CAP>
 static void move_pages(const PageArgs &a, const PageStep *steps, const uint32_t *ends, uint32_t lanes, uint32_t planes, cudaStream_t s) {
     PageMoves<CAP> m;
     m.a = a;
-    uint32_t longest = 0;
-    for (uint32_t i = 0; i < lanes; i++) {
-        m.end[i] = (uint16_t)ends[i];
-        longest = std::max(longest, ends[i] - (i ? ends[i - 1] : 0));
-    }
+    for (uint32_t i = 0; i < lanes; i++) m.end[i] = (uint16_t)ends[i];
     std::copy_n(steps, ends[lanes - 1], m.step);
-    const unsigned cols = a.half / 2;  // 32-byte columns of a page, a multiple of 2048
-    const auto go = [&](auto kernel, unsigned per) { launch_k(kernel, dim3(cols / (256 * per), lanes, planes), 256, 0, s, m); };
-    if (longest <= 1) go(pages_move_kernel<4, 1, CAP>, 4);
-    else if (longest <= 4) go(pages_move_kernel<2, 4, CAP>, 2);
-    else go(pages_move_kernel<1, 8, CAP>, 1);
+    // 32-byte columns of a page: half / 2, a multiple of 2048
+    launch_k(pages_move_kernel<CAP>, dim3(a.half / 512, lanes, planes), 256, 0, s, m);
 }
 
 void launch_pages_move(const PageArgs &a, const PageStep *steps, const uint32_t *ends, uint32_t lanes, uint32_t planes, cudaStream_t s) {
@@ -89,60 +73,62 @@ void launch_pages_move(const PageArgs &a, const PageStep *steps, const uint32_t 
 
 // ---- sum of products of ciphertexts ------------------------------------------------------------------------------------
 // out[g] = (sum_t a0 b0, sum_t a0 b1 + a1 b0, sum_t a1 b1) mod every prime: products of the pages with the scores that weigh them,
-// summed before any of them is relinearised. A thread owns V positions of a limb and walks the terms; sums stay in registers as
-// the prime's arithmetic likes them (sums.cuh) and are reduced once at the end. G queries share one read of the pages.
-template <class S, int G, int V, int U>
-__device__ __forceinline__ void multiply_sum_body(const SumArgs &a, const Mod &md) {
+// summed before any of them is relinearised. A thread owns one position of a limb and walks the terms, U of them loaded before the
+// first is multiplied; sums stay in registers as the prime's arithmetic likes them (sums.cuh) and are reduced once at the end.
+// G queries share one read of the pages.
+// Bound by HBM: 2 (G + 1) limbs a term for 4 G products. One word a thread and load keeps the sums of all arithmetics in 80 registers
+// (G = 1; 768 threads an SM with eight loads each in flight): 32 terms at N = 2^16, 16 limbs of 40 bits take 160.6 us (1.10 GB, 6.84
+// TB/s; 8.6 us for 17 terms of 6 limbs at 2^14), with two words a thread 168 to 193, with U = 8 and 128 registers 159.1, but 177.9
+// against 168.4 on primes of 55 bits. Four queries (24 pages at 2^15, 12 limbs, 0.79 GB): 129.9 us; 181 with each query's sums in
+// 21-bit pieces (72 registers of sums; FP64 products need 24 and take 131 to 137), and on integer primes, whose sums of 30-bit
+// pieces are wide too, the queries go two by two over the same pages: 186.2 against 187 to 259 at once. Terms dealt to four groups of
+// threads that join in shared memory gain 1.3 us of 10 at 60 terms and 96 CTAs and lose everywhere else: not built.
+constexpr int SUM_T = 128;
+template <class S, int G, int U>
+__device__ __forceinline__ void multiply_sum_body(const SumArgs &a, const Mod &md, uint32_t g0) {
+    constexpr int FULL = S::FLUSH / 2;  // terms that fill a sum: the middle one takes two products of each
+    static_assert(U <= FULL);
     const typename S::K k = S::make(md);
     const size_t N = (size_t)1 << a.logN;
-    const uint32_t limb = blockIdx.y, i = (blockIdx.x * 128 + threadIdx.x) * V;
-    const size_t o = (size_t)limb * N + i, ga = (size_t)a.la * N, gb = (size_t)a.lb * N;
-    typename S::Acc acc[G][3][V];
+    const size_t o = (size_t)blockIdx.y * N + blockIdx.x * SUM_T + threadIdx.x, ga = (size_t)a.la * N, gb = (size_t)a.lb * N;
+    typename S::Acc acc[G][3];
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
-        for (int p = 0; p < 3; p++)
-#pragma unroll
-            for (int j = 0; j < V; j++) S::zero(acc[g][p][j]);
+        for (int p = 0; p < 3; p++) S::zero(acc[g][p]);
     int pending = 0;
     for (uint32_t t = 0; t < a.terms; t += U) {
-        uint64_t b0[U][V], b1[U][V], a0[G][U][V], a1[G][U][V];
+        uint64_t b0[U], b1[U], a0[G][U], a1[G][U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (t + u < a.terms) {
-                ldv<V>(b0[u], a.b[t + u] + o), ldv<V>(b1[u], a.b[t + u] + gb + o);
+                b0[u] = a.b[t + u][o], b1[u] = a.b[t + u][gb + o];
 #pragma unroll
                 for (int g = 0; g < G; g++) {
-                    const uint64_t *x = a.a[g * a.terms + t + u] + o;
-                    ldv<V>(a0[g][u], x), ldv<V>(a1[g][u], x + ga);
+                    const uint64_t *x = a.a[(g0 + g) * a.terms + t + u] + o;
+                    a0[g][u] = x[0], a1[g][u] = x[ga];
                 }
             }
         }
-        // the middle sum takes two products a term
-        if (pending + 2 * U > S::FLUSH) {
+        if (pending + U > FULL) {
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll
-                for (int p = 0; p < 3; p++)
-#pragma unroll
-                    for (int j = 0; j < V; j++) S::flush(acc[g][p][j], k);
+                for (int p = 0; p < 3; p++) S::flush(acc[g][p], k);
             pending = 0;
         }
-        pending += 2 * U;
+        pending += U;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (t + u < a.terms) {
+                const typename S::A y0 = S::ld_a(b0[u], k), y1 = S::ld_a(b1[u], k);
 #pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const typename S::A y0 = S::ld_a(b0[u][j], k), y1 = S::ld_a(b1[u][j], k);
-#pragma unroll
-                    for (int g = 0; g < G; g++) {
-                        const typename S::B x0 = S::ld_b(a0[g][u][j], k), x1 = S::ld_b(a1[g][u][j], k);
-                        S::mac(acc[g][0][j], y0, x0, k);
-                        S::mac(acc[g][1][j], y1, x0, k);
-                        S::mac(acc[g][1][j], y0, x1, k);
-                        S::mac(acc[g][2][j], y1, x1, k);
-                    }
+                for (int g = 0; g < G; g++) {
+                    const typename S::B x0 = S::ld_b(a0[g][u], k), x1 = S::ld_b(a1[g][u], k);
+                    S::mac(acc[g][0], y0, x0, k);
+                    S::mac(acc[g][1], y1, x0, k);
+                    S::mac(acc[g][1], y0, x1, k);
+                    S::mac(acc[g][2], y1, x1, k);
                 }
             }
         }
@@ -151,34 +137,37 @@ __device__ __forceinline__ void multiply_sum_body(const SumArgs &a, const Mod &m
     for (int g = 0; g < G; g++)
 #pragma unroll
         for (int p = 0; p < 3; p++) {
-            uint64_t *out = a.out + ((size_t)(g * 3 + p) * a.l) * N + o;
-            uint64_t r[V];
-#pragma unroll
-            for (int j = 0; j < V; j++) r[j] = S::finish(acc[g][p][j], k);
-            if (!a.first) {
-                uint64_t was[V];
-                ldv<V>(was, out);
-#pragma unroll
-                for (int j = 0; j < V; j++) r[j] = add_mod(r[j], was[j], md.q);
-            }
-            stv<V>(out, r);
+            const uint64_t r = S::finish(acc[g][p], k);
+            uint64_t *out = a.out + (size_t)((g0 + g) * 3 + p) * a.l * N + o;
+            *out = a.first ? r : add_mod(r, *out, md.q);
         }
 }
 
-template <int G, int V, int U>
-__global__ void __launch_bounds__(128) multiply_sum_kernel(const __grid_constant__ SumArgs a) {
+template <int G, int U, int MIN_CTAS>
+__global__ void __launch_bounds__(SUM_T, MIN_CTAS) multiply_sum_kernel(const __grid_constant__ SumArgs a) {
     pdl_enter();
     const Mod md = a.mod[blockIdx.y];
-    with_sum(md.q, [&](auto s) { multiply_sum_body<decltype(s), G, V, U>(a, md); });
+    if constexpr (G <= 2) {
+        with_sum(md.q, [&](auto s) { multiply_sum_body<decltype(s), G, U>(a, md, 0); });
+    } else if (md.q < FP_LIMIT) {
+        multiply_sum_body<SumFp, G, U>(a, md, 0);
+    } else {
+        with_sum(md.q, [&](auto s) {
+            if constexpr (!std::is_same_v<decltype(s), SumFp> && !std::is_same_v<decltype(s), SumFp21>) {
+                multiply_sum_body<decltype(s), 2, U>(a, md, 0);
+                multiply_sum_body<decltype(s), G - 2, U>(a, md, 2);
+            }
+        });
+    }
 }
 
 void launch_multiply_sum(const SumArgs &a, uint32_t queries, cudaStream_t s) {
-    const auto go = [&](auto kernel, unsigned v) { launch_k(kernel, dim3((1u << a.logN) / (128 * v), a.l), 128, 0, s, a); };
+    const dim3 grid((1u << a.logN) / SUM_T, a.l);
     switch (queries) {
-        case 1: go(multiply_sum_kernel<1, 2, 2>, 2); break;
-        case 2: go(multiply_sum_kernel<2, 1, 2>, 1); break;
-        case 3: go(multiply_sum_kernel<3, 1, 2>, 1); break;
-        default: go(multiply_sum_kernel<4, 1, 2>, 1); break;
+        case 1: launch_k(multiply_sum_kernel<1, 4, 6>, grid, SUM_T, 0, s, a); break;
+        case 2: launch_k(multiply_sum_kernel<2, 3, 4>, grid, SUM_T, 0, s, a); break;
+        case 3: launch_k(multiply_sum_kernel<3, 3, 4>, grid, SUM_T, 0, s, a); break;
+        default: launch_k(multiply_sum_kernel<4, 3, 4>, grid, SUM_T, 0, s, a); break;
     }
 }
 

@@ -18,6 +18,7 @@ import enum
 import io
 import struct
 import threading
+from array import array
 
 import numpy as np
 import torch
@@ -577,42 +578,54 @@ def multiply_sum(ctx, a, b):
     at a time. No counterpart in the reference, which relinearises every product (src/attention.cu:60-90)."""
     if not len(b):
         raise ValueError("encrypteds cannot be empty")
-    first = _same_kind(ctx, b)
-    data = [ct.data.contiguous() for ct in b]
-    return _multiply_sum(ctx, a, np.array([t.data_ptr() for t in data], dtype=np.uint64), first._limbs, first._chain_index, first._scale)
+    first, table, held = _operands(ctx, [b])
+    return _multiply_sum(ctx, a, table, first._limbs, first._chain_index, first._scale)
 
 
-def _same_kind(ctx, cts):
-    first = cts[0]
-    for ct in cts:
-        if ct._chain_index != first._chain_index or ct._limbs != first._limbs or ct._N != ctx.N:
-            raise ValueError("encrypted1 and encrypted2 parameter mismatch")
-        if not ct._is_ntt_form:
-            raise ValueError("encrypted1 and encrypted2 must be in NTT form")
-        if ct._size != 2:
-            raise ValueError("only 2-polynomial operands are built")
-        if ct._scale != first._scale and not _are_close(ct._scale, first._scale):
-            raise ValueError("scale mismatch")
-    return first
+def _operands(ctx, rows):
+    """(the first ciphertext, the addresses of all as an array, copies of strided ones, which live until the launch)"""
+    first = rows[0][0]
+    chain_index, limbs, scale, N = first._chain_index, first._limbs, first._scale, ctx.N
+    addresses, held = array("Q"), []
+    for row in rows:
+        for ct in row:
+            if ct._chain_index != chain_index or ct._limbs != limbs or ct._N != N:
+                raise ValueError("encrypted1 and encrypted2 parameter mismatch")
+            if not ct._is_ntt_form:
+                raise ValueError("encrypted1 and encrypted2 must be in NTT form")
+            if ct._size != 2:
+                raise ValueError("only 2-polynomial operands are built")
+            if ct._scale != scale and not _are_close(ct._scale, scale):
+                raise ValueError("scale mismatch")
+            data = ct.data
+            if not data.is_contiguous():
+                data = data.contiguous()
+                held.append(data)
+            addresses.append(data.data_ptr())
+    return first, addresses, held
 
 
 def _multiply_sum(ctx, a, table, b_limbs, b_chain_index, b_scale):
     """a: a list of ciphertexts or a list of such lists; table: the addresses of the other operands"""
+    terms = len(table)
     if not len(a):
         raise ValueError("encrypteds cannot be empty")
     many = isinstance(a[0], (list, tuple))
     rows = a if many else [a]
-    if any(len(r) != len(table) for r in rows) or not len(table):
+    if not terms or any(len(r) != terms for r in rows):
         raise ValueError("multiply_sum: as many ciphertexts in every list are wanted, and at least one")
-    cts = [ct for r in rows for ct in r]
-    first = _same_kind(ctx, cts)
-    held = [ct.data.contiguous() for ct in cts]  # strided views become copies, which live until the launch
-    tab = np.array([t.data_ptr() for t in held], dtype=np.uint64)
+    first, addresses, held = _operands(ctx, rows)
     l = min(first._limbs, b_limbs)
-    out = ctx.empty(len(rows), 3, l)
+    out = torch.empty(len(rows), 3, l, ctx.N, dtype=torch.int64, device=ctx.device)
     with _native.on_device(ctx):
-        check(LIB.b2_multiply_sum(ctx._h, l, len(rows), len(table), tab.ctypes.data, first._limbs, table.ctypes.data, b_limbs, out.data_ptr(), _stream()))
-    res = [first._like(out[g], chain_index=max(first._chain_index, b_chain_index), scale=first._scale * b_scale) for g in range(len(rows))]
+        check(LIB.b2_multiply_sum(ctx._h, l, len(rows), terms, addresses.buffer_info()[0], first._limbs, table.buffer_info()[0], b_limbs, out.data_ptr(),
+                                  _stream()))
+    res = []
+    for data in out.unbind(0):
+        ct = ciphertext.__new__(ciphertext)
+        ct.__dict__.update(first.__dict__)
+        ct._size, ct._limbs, ct._chain_index, ct._scale, ct.data = 3, l, max(first._chain_index, b_chain_index), first._scale * b_scale, data
+        res.append(ct)
     return res if many else res[0]
 
 

@@ -136,8 +136,9 @@ current_stream = _stream_lookup()
 
 
 _NOTHING = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def on_device(ctx):
     """a context manager that makes the context's device the current one, so that current_stream() is a stream of it"""
-    return _NOTHING if torch.cuda.current_device() == ctx.device else torch.cuda.device(ctx.device)
+    return _NOTHING if _current_device() == ctx.device else torch.cuda.device(ctx.device)

@@ -11,6 +11,7 @@ stream at a time; calls work on torch's current stream of the context's device. 
 replays the moves of the numbers it was captured with.
 """
 import heapq
+from array import array
 
 import numpy as np
 import torch
@@ -27,6 +28,7 @@ class ciphertext_cache:
         if not 1 <= chain_index <= context.size_Q:
             raise ValueError("chain index out of range")
         self.ctx, self._chain_index, self._limbs, self._scale = context, int(chain_index), context.limbs_at(chain_index), float(scale)
+        self._planes, self._page_bytes = planes, 16 * self._limbs * context.N
         self.data = context.empty(planes, pages, 2, self._limbs)
         self._held = [0] * pages       # how many tables hold a page
         self._free = list(range(pages))  # a heap: the lowest number goes out first
@@ -39,7 +41,7 @@ class ciphertext_cache:
         return self._scale
 
     def planes(self):
-        return self.data.shape[0]
+        return self._planes
 
     def pages(self):
         return len(self._held)
@@ -58,13 +60,22 @@ class ciphertext_cache:
         return page
 
     def _live(self, pages):
-        pages = [self._number(p) for p in pages]
-        if not all(self._held[p] for p in pages):
+        """the page numbers as a list, each of an allocated page"""
+        if type(pages) is not list:
+            pages = [int(p) for p in pages]
+        held = self._held
+        try:
+            ok = not pages or (min(pages) >= 0 and all(map(held.__getitem__, pages)))
+        except IndexError:
+            ok = False
+        if not ok:
+            for p in pages:
+                self._number(p)
             raise ValueError("ciphertext_cache: page is not allocated")
         return pages
 
     def _plane(self, plane):
-        if not 0 <= int(plane) < self.data.shape[0]:
+        if not 0 <= int(plane) < self._planes:
             raise ValueError("ciphertext_cache: plane out of range")
         return int(plane)
 
@@ -85,13 +96,14 @@ class ciphertext_cache:
 
     # ---- pages ------------------------------------------------------------------------------------------------------
     def _move(self, dst, src, source=None):
-        if not len(dst):
+        n = len(dst)
+        if not n:
             return
-        d, s = np.array(dst, dtype=np.int64), np.array(src, dtype=np.int64)
-        x = self.data if source is None else source.data
+        d, s = array("q", dst), array("q", src)  # half the host time of numpy arrays
+        x = self if source is None else source
         with on_device(self.ctx):
-            check(LIB.b2_pages_move(self.ctx._h, self._limbs, self.data.shape[0], self.data.data_ptr(), len(self._held), x.data_ptr(), x.shape[3],
-                                    x.shape[1], len(d), d.ctypes.data, s.ctypes.data, _stream()))
+            check(LIB.b2_pages_move(self.ctx._h, self._limbs, self._planes, self.data.data_ptr(), len(self._held), x.data.data_ptr(), x._limbs,
+                                    len(x._held), n, d.buffer_info()[0], s.buffer_info()[0], _stream()))
 
     def allocate(self, n=1):
         """n pages that nobody holds, as a table; zeros in every plane"""
@@ -151,7 +163,7 @@ class ciphertext_cache:
         if len(dst) != len(src):
             raise ValueError("ciphertext_cache: as many sources as destinations are wanted")
         other = self if source is None else source
-        if other.ctx is not self.ctx or other.planes() != self.planes() or other._limbs < self._limbs:
+        if other.ctx is not self.ctx or other._planes != self._planes or other._limbs < self._limbs:
             raise ValueError("ciphertext_cache: the source has another context, other planes or a lower level")
         self._move(self._live(dst), other._live(src), source)
 
@@ -174,14 +186,14 @@ class ciphertext_cache:
         pages = int(pages)
         if pages < 1 or any(self._held[pages:]):
             raise ValueError("ciphertext_cache: allocated pages lie behind the new end (compact first)")
-        old, n = self.data, min(pages, len(self._held))
-        live = [p for p in range(n) if self._held[p]]
-        data = self.ctx.empty(old.shape[0], pages, 2, self._limbs)
-        d = np.array(live, dtype=np.int64)
+        n = min(pages, len(self._held))
+        data = self.ctx.empty(self._planes, pages, 2, self._limbs)
+        live = array("q", [p for p in range(n) if self._held[p]])
         if live:
+            at = live.buffer_info()[0]
             with on_device(self.ctx):
-                check(LIB.b2_pages_move(self.ctx._h, self._limbs, old.shape[0], data.data_ptr(), pages, old.data_ptr(), self._limbs, old.shape[1],
-                                        len(d), d.ctypes.data, d.ctypes.data, _stream()))
+                check(LIB.b2_pages_move(self.ctx._h, self._limbs, self._planes, data.data_ptr(), pages, self.data.data_ptr(), self._limbs, len(self._held),
+                                        len(live), at, at, _stream()))
         self.data = data
         self._held = self._held[:n] + [0] * (pages - n)
         self._free = [p for p, k in enumerate(self._held) if not k]
@@ -215,9 +227,9 @@ class ciphertext_cache:
         """multiply_sum of `scores` with the pages, read where they lie: sum_t scores[t] x page[pages[t]] as one three-polynomial
         ciphertext at the lower of the two levels. A list of such lists (queries that read the same pages) gives a list."""
         pages = self._live(pages)
-        base, step = self.data[self._plane(plane)].data_ptr(), 16 * self._limbs * self.ctx.N
-        table = np.array(pages, dtype=np.uint64) * np.uint64(step) + np.uint64(base)
-        return _multiply_sum(self.ctx, scores, table, self._limbs, self._chain_index, self._scale)
+        step = self._page_bytes
+        base = self.data.data_ptr() + self._plane(plane) * len(self._held) * step
+        return _multiply_sum(self.ctx, scores, array("Q", [base + p * step for p in pages]), self._limbs, self._chain_index, self._scale)
 
 
 # ---- attention products ---------------------------------------------------------------------------------------------------
@@ -259,7 +271,8 @@ def cached_qkt(context, relin_key, galois_key, q, cache, pages, d_head, plane=0)
     l, nominal, results = q._limbs, q._scale, []
     tab = _key_table(ctx, relin_key, l)
     x = q.data.contiguous()
-    base, step = cache.data[plane].data_ptr(), 16 * cache._limbs * ctx.N
+    step = cache._page_bytes
+    base = cache.data.data_ptr() + plane * cache.pages() * step
     with on_device(ctx):
         for p0 in range(0, len(pages), BATCH):
             part = pages[p0:p0 + BATCH]

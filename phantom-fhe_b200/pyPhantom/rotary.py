@@ -43,28 +43,28 @@ class rotary:
         self.positions_per_ct = context.N // 2 // (heads * d_head)
         self.inv_freq, self.axes = f, torch.tensor(a, dtype=torch.int32, device=context.device)
         self.step = pairs if packing == "halves" else 1
+        self._vecs = 1 if packing == "pairs" else 3
 
     def factors(self, positions, keep=None, conjugate=False):
         """The factors of `positions` ([tokens] or [tokens][axes], int32, int64, float32 or float64, any strides) as complex128
         [vectors][ciphertexts][slots], one vector ("pairs") or three (C, A, B), positions_per_ct tokens to a ciphertext. keep: bool
         [tokens], False for a token whose slots become zeros. conjugate: the inverse rotation."""
-        ctx, p = self.ctx, positions
-        if p.dim() == 1:
-            p = p.unsqueeze(1)
-        if p.dim() != 2 or p.dtype not in _POSITIONS:
+        ctx, p, dims = self.ctx, positions, positions.dim()
+        kind = _POSITIONS.get(p.dtype)
+        if not 1 <= dims <= 2 or kind is None:
             raise ValueError("rotary: positions are [tokens] or [tokens][axes] of int32, int64, float32 or float64")
-        if p.shape[1] < self.n_axes:
+        tokens = p.shape[0]
+        if (p.shape[1] if dims == 2 else 1) < self.n_axes:
             raise ValueError("rotary: positions have fewer axes than the pairs name")
-        if keep is not None and (keep.dtype != torch.bool or keep.dim() != 1 or keep.shape[0] != p.shape[0]):
+        if keep is not None and (keep.dtype != torch.bool or keep.dim() != 1 or keep.shape[0] != tokens):
             raise ValueError("rotary: keep is one truth value a token")
         if p.get_device() != ctx.device or (keep is not None and keep.get_device() != ctx.device):
             raise ValueError("rotary: positions and keep must lie on the context's device")
-        tokens = p.shape[0]
-        out = torch.empty(1 if self.packing == "pairs" else 3, -(-tokens // self.positions_per_ct), ctx.N // 2, dtype=torch.complex128, device=ctx.device)
+        out = torch.empty(self._vecs, -(-tokens // self.positions_per_ct), ctx.N // 2, dtype=torch.complex128, device=ctx.device)
         with on_device(ctx):
-            check(LIB.b2_rotary_factors(ctx._h, _PACKINGS[self.packing], tokens, self.heads, self.d_head, self.pairs, p.data_ptr(), _POSITIONS[p.dtype],
-                                        p.stride(0), p.stride(1), self.inv_freq.data_ptr(), self.axes.data_ptr(), 0 if keep is None else keep.data_ptr(),
-                                        0 if keep is None else keep.stride(0), self.scaling, int(bool(conjugate)), out.data_ptr(), _stream()))
+            check(LIB.b2_rotary_factors(ctx._h, _PACKINGS[self.packing], tokens, self.heads, self.d_head, self.pairs, p.data_ptr(), kind, p.stride(0),
+                                        p.stride(1) if dims == 2 else 0, self.inv_freq.data_ptr(), self.axes.data_ptr(), 0 if keep is None else keep.data_ptr(),
+                                        0 if keep is None else keep.stride(0), self.scaling, 1 if conjugate else 0, out.data_ptr(), _stream()))
         return out
 
     def encode(self, encoder, factors, chain_index):
@@ -102,7 +102,7 @@ class rotary:
         """the ciphertexts xs rotated by the encoded factors, one level further down (rounded to nearest), at their scale. "halves" and "interleaved"
         want a Galois key for the steps +-`step`."""
         ctx = self.ctx
-        vecs = 1 if self.packing == "pairs" else 3
+        vecs = self._vecs
         if len(plaintexts) != vecs or any(len(v) != len(xs) for v in plaintexts):
             raise ValueError("rotary: as many encoded factors as ciphertexts are wanted")
         if vecs == 3 and xs and galois_key is None:
