@@ -153,12 +153,15 @@ int b2_sample(b2_ctx *ctx, int kind, const uint8_t *key32, const uint8_t *nonce1
 /* Encoding, symmetric encryption, decryption and decoding as one call each (src/ckks.cu:68-190, src/secretkey.cu:236-299,
  * 883-919); the tables are those of b2_special_fft and b2_decode_compose.
  *   b2_encode_coeffs:     d_vals (N/2 complex values, overwritten) -> d_coeffs int64 [N], each below 2^62 in magnitude
+ *   b2_encode_coeffs_batch: M of them, one behind the other: d_vals [M][N/2], d_coeffs [M][N], two launches for all
  *   b2_encrypt_symmetric: d_out [2][l][N] = (m - (a s + e), a); a and e from the key and nonce (32 + 12 bytes) given for
  *                         each; d_sk [l][N]; d_pt [l][N] or null; d_ws N words
  *   b2_decrypt:           d_out [l][N] = c0 + c1 s
  *   b2_decode_slots:      d_pt [l][N] -> d_out N/2 complex values; d_ws (l + 1) N words */
 int b2_encode_coeffs(b2_ctx *ctx, void *d_vals, const uint32_t *d_rot, const void *d_ksi, double scale,
                      int64_t *d_coeffs, void *stream);
+int b2_encode_coeffs_batch(b2_ctx *ctx, size_t M, void *d_vals, const uint32_t *d_rot, const void *d_ksi, double scale,
+                           int64_t *d_coeffs, void *stream);
 int b2_encrypt_symmetric(b2_ctx *ctx, size_t l, const uint8_t *mask44, const uint8_t *error44, const uint64_t *d_sk,
                          const uint64_t *d_pt, uint64_t *d_out, void *d_ws, void *stream);
 int b2_decrypt(b2_ctx *ctx, size_t l, const uint64_t *d_ct, const uint64_t *d_sk, uint64_t *d_out, void *stream);
@@ -346,6 +349,11 @@ int b2_pages_move(b2_ctx *ctx, size_t limbs, size_t planes, uint64_t *d_pool, si
  * from the operands. */
 int b2_multiply_sum(b2_ctx *ctx, size_t size_Ql, size_t queries, size_t terms, const uint64_t *const *d_a, size_t a_limbs,
                     const uint64_t *const *d_b, size_t b_limbs, uint64_t *d_out, void *stream);
+/* b2_multiply_plain_sum: out[i] = sum_t ct[i * terms + t] times pt[i * terms + t] (multiply_plain and add, src/evaluate.cu:1150-1200)
+ * for n ciphertexts in one launch, 1 to 4 terms; HOST arrays of n * terms device pointers to [2][size_Ql][N] and [size_Ql][N];
+ * d_out [n][2][size_Ql][N], apart from the operands. */
+int b2_multiply_plain_sum(b2_ctx *ctx, size_t size_Ql, size_t n, size_t terms, const uint64_t *const *d_ct,
+                          const uint64_t *const *d_pt, uint64_t *d_out, void *stream);
 /* b2_rotary_factors: the slot values by which a ciphertext of `per` = slots / (heads * d_head) positions is rotated, for `tokens`
  * positions in ceil(tokens / per) ciphertexts: theta[t][j] = position[t][axis[j]] * inv_freq[j] (rounded to a double), slot
  * (t mod per) * heads * d_head + h * d_head + i of ciphertext t / per.

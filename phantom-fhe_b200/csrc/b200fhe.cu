@@ -2354,8 +2354,10 @@ extern "C" int b2_expand_signed(b2_ctx *c, size_t first_prime, size_t n_limbs, c
 }
 
 // passes of the encoder's transform: n = 2^logn values as 2^(logn / 2) columns' worth of rows (8 stages a pass at most)
-static void run_cfft_inverse(const b2_ctx *c, double2 *v, double2 *out, int64_t *coeffs, const uint32_t *rot, const double2 *ksi, double scale, cudaStream_t s) {
-    const uint32_t logn = (uint32_t)c->logN - 1, la = logn / 2, lb = logn - la, grid = 1u << (logn - CFFT_LOG_TILE);
+static void run_cfft_inverse(const b2_ctx *c, double2 *v, double2 *out, int64_t *coeffs, const uint32_t *rot, const double2 *ksi, double scale, cudaStream_t s,
+                             uint32_t vectors = 1) {
+    const uint32_t logn = (uint32_t)c->logN - 1, la = logn / 2, lb = logn - la;
+    const dim3 grid(1u << (logn - CFFT_LOG_TILE), vectors);
     launch_k(cfft_pass_kernel<true, true, false>, grid, 512, 0, s, v, v, nullptr, logn, la, rot, ksi, 1.0);
     if (coeffs) launch_k(cfft_pass_kernel<true, false, true>, grid, 512, 0, s, v, nullptr, coeffs, logn, lb, rot, ksi, scale);
     else launch_k(cfft_pass_kernel<true, false, false>, grid, 512, 0, s, v, out, nullptr, logn, lb, rot, ksi, scale);
@@ -2388,6 +2390,18 @@ extern "C" int b2_encode_coeffs(b2_ctx *c, void *d_vals, const uint32_t *d_rot, 
     if (!d_vals || !d_rot || !d_ksi || !d_coeffs) return fail(B2_EINVAL, "encode_coeffs: null pointer");
     LaunchScope ls(c, (cudaStream_t)stream, "special_fft");
     run_cfft_inverse(c, (double2 *)d_vals, nullptr, d_coeffs, d_rot, (const double2 *)d_ksi, scale, (cudaStream_t)stream);
+    LAUNCH_CHECK("special_fft kernels");
+    return B2_OK;
+}
+
+extern "C" int b2_encode_coeffs_batch(b2_ctx *c, size_t M, void *d_vals, const uint32_t *d_rot, const void *d_ksi, double scale, int64_t *d_coeffs, void *stream) {
+    CHECK_CTX(c);
+    if (!d_vals || !d_rot || !d_ksi || !d_coeffs || M == 0) return fail(B2_EINVAL, "encode_coeffs_batch: bad argument");
+    for (size_t m = 0; m < M; m += 65535) {  // the vectors are the grid's second dimension
+        LaunchScope ls(c, (cudaStream_t)stream, "special_fft");
+        run_cfft_inverse(c, (double2 *)d_vals + m * (c->N / 2), nullptr, d_coeffs + m * c->N, d_rot, (const double2 *)d_ksi, scale, (cudaStream_t)stream,
+                         (uint32_t)std::min<size_t>(M - m, 65535));
+    }
     LAUNCH_CHECK("special_fft kernels");
     return B2_OK;
 }
@@ -2633,6 +2647,7 @@ extern "C" int b2_pages_move(b2_ctx *c, size_t limbs, size_t planes, uint64_t *d
     CHECK_CTX(c);
     CHECK_LEVEL(c, limbs);
     const bool apart = d_src && d_src != d_pool;
+    if (d_src == d_pool && (src_limbs != limbs || src_pages != pages)) return fail(B2_EINVAL, "pages_move: the source is the pool and has another shape");
     if (!apart) d_src = d_pool, src_limbs = limbs, src_pages = pages;
     if (!d_pool || (n && (!dst || !src))) return fail(B2_EINVAL, "pages_move: null pointer");
     if (planes < 1 || planes > 65535 || pages < 1 || pages > PAGE_MAX || src_pages < 1 || src_pages > PAGE_MAX)
@@ -2679,6 +2694,10 @@ extern "C" int b2_multiply_sum(b2_ctx *c, size_t l, size_t queries, size_t terms
     for (size_t i = 0; i < queries * terms; i++) ok = ok && d_a[i] && aligned32(d_a[i]);
     for (size_t i = 0; i < terms; i++) ok = ok && d_b[i] && aligned32(d_b[i]);
     if (!ok) return fail(B2_EINVAL, "multiply_sum: operands must be there and 32-byte aligned");
+    const auto overlaps = [&](const uint64_t *x, size_t limbs) { return x < d_out + queries * 3 * l * c->N && d_out < x + 2 * limbs * c->N; };
+    for (size_t i = 0; i < queries * terms; i++) ok = ok && !overlaps(d_a[i], la);
+    for (size_t i = 0; i < terms; i++) ok = ok && !overlaps(d_b[i], lb);
+    if (!ok) return fail(B2_EINVAL, "multiply_sum: the result overlaps an operand");
     for (size_t q0 = 0; q0 < queries; q0 += SUM_QUERIES) {
         const size_t g = std::min<size_t>(SUM_QUERIES, queries - q0);
         for (size_t t0 = 0; t0 < terms; t0 += SUM_TERMS) {
@@ -2693,6 +2712,27 @@ extern "C" int b2_multiply_sum(b2_ctx *c, size_t l, size_t queries, size_t terms
         }
     }
     LAUNCH_CHECK("multiply_sum_kernel");
+    return B2_OK;
+}
+
+extern "C" int b2_multiply_plain_sum(b2_ctx *c, size_t l, size_t n, size_t terms, const uint64_t *const *d_ct, const uint64_t *const *d_pt, uint64_t *d_out,
+                                     void *stream) {
+    CHECK_CTX(c);
+    CHECK_LEVEL(c, l);
+    if (!d_ct || !d_pt || !d_out || n < 1 || terms < 1 || terms > (size_t)PLAIN_TERMS) return fail(B2_EINVAL, "multiply_plain_sum: bad argument (1 to 4 terms)");
+    bool ok = aligned32(d_out);
+    for (size_t i = 0; i < n * terms; i++) ok = ok && d_ct[i] && d_pt[i] && aligned32(d_ct[i]) && aligned32(d_pt[i]);
+    if (!ok) return fail(B2_EINVAL, "multiply_plain_sum: operands must be there and 32-byte aligned");
+    for (size_t i = 0; i < n; i += PLAIN_SETS) {
+        const size_t m = std::min<size_t>(PLAIN_SETS, n - i);
+        PlainSumArgs a{};
+        a.out = d_out + i * 2 * l * c->N, a.mod = c->d_mod, a.logN = (uint32_t)c->logN, a.l = (uint32_t)l, a.terms = (uint32_t)terms;
+        std::copy_n(d_ct + i * terms, m * terms, a.ct);
+        std::copy_n(d_pt + i * terms, m * terms, a.pt);
+        LaunchScope ls(c, (cudaStream_t)stream, "multiply_plain_sum");
+        launch_multiply_plain_sum(a, (uint32_t)m, (cudaStream_t)stream);
+    }
+    LAUNCH_CHECK("multiply_plain_sum_kernel");
     return B2_OK;
 }
 

@@ -171,6 +171,55 @@ void launch_multiply_sum(const SumArgs &a, uint32_t queries, cudaStream_t s) {
     }
 }
 
+// ---- sums of ciphertexts times plaintexts ---------------------------------------------------------------------------------
+// out[z] = sum_t ct[z][t] (.) pt[z][t], t below 4: what a rotated ciphertext is (x C + rot(x, s) A + rot(x, -s) B), for a batch of
+// them in one launch. Bound by HBM: 3 limbs a term and 2.
+template <class S>
+__device__ __forceinline__ void plain_sum_body(const PlainSumArgs &a, const Mod &md) {
+    const typename S::K k = S::make(md);
+    const size_t N = (size_t)1 << a.logN, o = (size_t)blockIdx.y * N + (blockIdx.x * 128 + threadIdx.x) * 2, P = (size_t)a.l * N;
+    const uint32_t z = blockIdx.z;
+    typename S::Acc acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) S::zero(acc[i][0]), S::zero(acc[i][1]);
+    uint64_t x[PLAIN_TERMS][2], y[PLAIN_TERMS][2][2];
+#pragma unroll
+    for (int t = 0; t < PLAIN_TERMS; t++) {
+        if (t < (int)a.terms) {
+            ldv<2>(x[t], a.pt[z * a.terms + t] + o);
+            const uint64_t *c = a.ct[z * a.terms + t] + o;
+            ldv<2>(y[t][0], c), ldv<2>(y[t][1], c + P);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < PLAIN_TERMS; t++) {
+        if (t < (int)a.terms) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const typename S::A w = S::ld_a(x[t][j], k);
+                S::mac(acc[0][j], w, S::ld_b(y[t][0][j], k), k);
+                S::mac(acc[1][j], w, S::ld_b(y[t][1][j], k), k);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint64_t r[2] = {S::finish(acc[i][0], k), S::finish(acc[i][1], k)};
+        stv<2>(a.out + (size_t)z * 2 * P + i * P + o, r);
+    }
+}
+__global__ void __launch_bounds__(128) multiply_plain_sum_kernel(const __grid_constant__ PlainSumArgs a) {
+    pdl_enter();
+    const Mod md = a.mod[blockIdx.y];
+    if (md.q < FP_LIMIT) plain_sum_body<SumFp>(a, md);
+    else if (md.q < INT_LAZY_LIMIT) plain_sum_body<SumInt30Short>(a, md);
+    else plain_sum_body<SumInt>(a, md);
+}
+
+void launch_multiply_plain_sum(const PlainSumArgs &a, uint32_t sets, cudaStream_t s) {
+    launch_k(multiply_plain_sum_kernel, dim3((1u << a.logN) / 256, a.l, sets), 128, 0, s, a);
+}
+
 // ---- rotary positions ----------------------------------------------------------------------------------------------------
 // theta[t][j] = position[t][axis[j]] inv_freq[j], rounded once, then (cos, sin) in every head of the position's block of slots.
 // blockIdx.x = block of d_total slots (token), blockIdx.y = a share of its heads. A thread owns one slot of a head (in `rows` heads

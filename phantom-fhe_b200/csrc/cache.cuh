@@ -34,6 +34,17 @@ struct SumArgs {
 };
 void launch_multiply_sum(const SumArgs &a, uint32_t queries, cudaStream_t s);
 
+// ---- sums of ciphertexts times plaintexts, several at once ----------------------------------------------------------------
+constexpr int PLAIN_TERMS = 4, PLAIN_SETS = 32;
+struct PlainSumArgs {
+    uint64_t *out;                  // [sets][2][l][N]
+    const Mod *mod;
+    uint32_t logN, l, terms;
+    const uint64_t *ct[PLAIN_SETS * PLAIN_TERMS];  // [set][terms], [2][l][N] each
+    const uint64_t *pt[PLAIN_SETS * PLAIN_TERMS];  // [l][N]
+};
+void launch_multiply_plain_sum(const PlainSumArgs &a, uint32_t sets, cudaStream_t s);
+
 // ---- rotary positions ---------------------------------------------------------------------------------------------------
 enum { ROTARY_PAIRS = 0, ROTARY_HALVES = 1, ROTARY_INTERLEAVED = 2 };
 struct RotaryArgs {

@@ -31,12 +31,14 @@ __device__ __forceinline__ double2 cmul(double2 a, double2 b) {
 //   INVERSE (encode): strided pass (len = n .. 2 n / T), then the contiguous one, results bit-reversed and scaled;
 //   forward (decode): contiguous pass on bit-reversed, scaled input, then the strided one.
 // ROUND: the last inverse pass writes rint(Re) to coeffs[k] and rint(Im) to coeffs[k + n] instead of complex values.
+// blockIdx.y: vector of a batch, one behind the other.
 constexpr int CFFT_LOG_TILE = 10, CFFT_MAX_STAGES = 8;
 template <bool INVERSE, bool STRIDED, bool ROUND>
 __global__ void __launch_bounds__(512) cfft_pass_kernel(const double2 *in, double2 *out, int64_t *coeffs, uint32_t logn, uint32_t logT,
                                                         const uint32_t *__restrict__ rot, const double2 *__restrict__ ksi, double k) {
     pdl_enter();
     __shared__ double2 sm[1 << CFFT_LOG_TILE];
+    in += (size_t)blockIdx.y << logn, out += (size_t)blockIdx.y << logn, coeffs += (size_t)blockIdx.y << (logn + 1);  // vector of a batch
     const uint32_t n = 1u << logn, log_other = logn - logT, logC = CFFT_LOG_TILE - logT, C = 1u << logC, T = 1u << logT;
     const uint32_t tid = threadIdx.x, tile = blockIdx.x;
     // shared position p of the tile <-> index of the transform: [e][c] strided, [c][e] contiguous

@@ -585,7 +585,9 @@ def multiply_sum(ctx, a, b):
 def _operands(ctx, rows):
     """(the first ciphertext, the addresses of all as an array, copies of strided ones, which live until the launch)"""
     first = rows[0][0]
-    chain_index, limbs, scale, N = first._chain_index, first._limbs, first._scale, ctx.N
+    chain_index, limbs, scale, N, device = first._chain_index, first._limbs, first._scale, ctx.N, ctx.device
+    if chain_index < 1 or limbs != ctx.limbs_at(chain_index):
+        raise ValueError("encrypted1 and encrypted2 parameter mismatch")
     addresses, held = array("Q"), []
     for row in rows:
         for ct in row:
@@ -598,6 +600,8 @@ def _operands(ctx, rows):
             if ct._scale != scale and not _are_close(ct._scale, scale):
                 raise ValueError("scale mismatch")
             data = ct.data
+            if data.numel() != 2 * limbs * N or data.dtype != torch.int64 or data.get_device() != device:
+                raise ValueError("the ciphertext's words are not on the context's device, or not as many as its level has")
             if not data.is_contiguous():
                 data = data.contiguous()
                 held.append(data)
@@ -612,16 +616,22 @@ def _multiply_sum(ctx, a, table, b_limbs, b_chain_index, b_scale):
         raise ValueError("encrypteds cannot be empty")
     many = isinstance(a[0], (list, tuple))
     rows = a if many else [a]
-    if not terms or any(len(r) != terms for r in rows):
-        raise ValueError("multiply_sum: as many ciphertexts in every list are wanted, and at least one")
+    for r in rows:
+        if not terms or len(r) != terms:
+            raise ValueError("multiply_sum: as many ciphertexts in every list are wanted, and at least one")
     first, addresses, held = _operands(ctx, rows)
     l = min(first._limbs, b_limbs)
-    out = torch.empty(len(rows), 3, l, ctx.N, dtype=torch.int64, device=ctx.device)
+    if len(rows) == 1:  # a view less
+        out = torch.empty(3, l, ctx.N, dtype=torch.int64, device=ctx.device)
+        results = (out,)
+    else:
+        out = torch.empty(len(rows), 3, l, ctx.N, dtype=torch.int64, device=ctx.device)
+        results = out.unbind(0)
     with _native.on_device(ctx):
         check(LIB.b2_multiply_sum(ctx._h, l, len(rows), terms, addresses.buffer_info()[0], first._limbs, table.buffer_info()[0], b_limbs, out.data_ptr(),
                                   _stream()))
     res = []
-    for data in out.unbind(0):
+    for data in results:
         ct = ciphertext.__new__(ciphertext)
         ct.__dict__.update(first.__dict__)
         ct._size, ct._limbs, ct._chain_index, ct._scale, ct.data = 3, l, max(first._chain_index, b_chain_index), first._scale * b_scale, data

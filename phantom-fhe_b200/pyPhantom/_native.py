@@ -49,6 +49,7 @@ SIGNATURES = {
     "b2_peer_copy": (_int, [_vp, _vp, _sz, _vp]),
     "b2_sample": (_int, [_vp, _int, _vp, _vp, _sz, _sz, _vp, _vp]),
     "b2_encode_coeffs": (_int, [_vp, _vp, _vp, _vp, ctypes.c_double, _vp, _vp]),
+    "b2_encode_coeffs_batch": (_int, [_vp, _sz, _vp, _vp, _vp, ctypes.c_double, _vp, _vp]),
     "b2_encrypt_symmetric": (_int, [_vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b2_decrypt": (_int, [_vp, _sz, _vp, _vp, _vp, _vp]),
     "b2_decode_slots": (_int, [_vp, _sz, _vp, _vp, ctypes.c_double, _vp, _vp, _vp, _vp, _vp]),
@@ -82,6 +83,7 @@ SIGNATURES = {
     "b2_poly_scalar": (_int, [_vp, _int, _sz, _vp, _vp, _vp, _vp]),
     "b2_pages_move": (_int, [_vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _vp, _vp]),
     "b2_multiply_sum": (_int, [_vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp]),
+    "b2_multiply_plain_sum": (_int, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
     "b2_rotary_factors": (_int, [_vp, _int, _sz, _sz, _sz, _sz, _vp, _int, _i64, _i64, _vp, _vp, _vp, _i64, ctypes.c_double, _int, _vp, _vp]),
     "b2_ctx_set_shard": (_int, [_vp, _int, _int]),
     "b2_shard_limbs": (_int, [_vp, _sz, _vp]),

@@ -16,7 +16,7 @@ from array import array
 import numpy as np
 import torch
 
-from . import _check_plain, _galois_index, _key_table, _multiply_sum, _rescale_rounded, add, ciphertext, get_elt_from_step, relinearize, rotate
+from . import _check_plain, _galois_index, _key_table, _multiply_sum, _operands, _rescale_rounded, add, ciphertext, get_elt_from_step, relinearize, rotate
 from ._native import LIB, check, current_stream as _stream, on_device
 
 
@@ -165,7 +165,10 @@ class ciphertext_cache:
         other = self if source is None else source
         if other.ctx is not self.ctx or other._planes != self._planes or other._limbs < self._limbs:
             raise ValueError("ciphertext_cache: the source has another context, other planes or a lower level")
-        self._move(self._live(dst), other._live(src), source)
+        dst = self._live(dst)
+        if any(self._held[p] > 1 for p in dst):
+            raise ValueError("ciphertext_cache: the page is shared (fork the table first)")
+        self._move(dst, other._live(src), source)
 
     def compact(self, tables):
         """Moves all allocated pages to the front of the pool, those of `tables` first and in their order (a table's pages then
@@ -203,8 +206,8 @@ class ciphertext_cache:
         (page,) = self._live([page])
         if self._held[page] > 1:
             raise ValueError("ciphertext_cache: the page is shared (fork the table first)")
-        if ct._size != 2 or not ct._is_ntt_form or ct._N != self.ctx.N:
-            raise ValueError("ciphertext_cache: a two-polynomial ciphertext in NTT form is wanted")
+        if ct._size != 2 or not ct._is_ntt_form or ct.data.shape != (2, ct._limbs, self.ctx.N) or ct.data.get_device() != self.ctx.device:
+            raise ValueError("ciphertext_cache: a two-polynomial ciphertext in NTT form on the context's device is wanted")
         if ct._chain_index > self._chain_index:
             raise ValueError("cannot switch to higher level modulus")
         if abs(ct._scale - self._scale) > 1e-9 * self._scale:
@@ -264,20 +267,18 @@ def cached_qkt(context, relin_key, galois_key, q, cache, pages, d_head, plane=0)
         raise ValueError("ciphertext_cache: the cache belongs to another context")
     if q._chain_index < cache._chain_index:
         raise ValueError("encrypted1 and encrypted2 parameter mismatch")
-    if q._size != 2 or not q._is_ntt_form:
-        raise ValueError("only 2-polynomial operands in NTT form are built")
+    _, table, held = _operands(ctx, [[q]])
     if q._chain_index == ctx.size_Q:
         raise ValueError("end of modulus switching chain reached")
     l, nominal, results = q._limbs, q._scale, []
     tab = _key_table(ctx, relin_key, l)
-    x = q.data.contiguous()
     step = cache._page_bytes
     base = cache.data.data_ptr() + plane * cache.pages() * step
     with on_device(ctx):
         for p0 in range(0, len(pages), BATCH):
             part = pages[p0:p0 + BATCH]
             n = len(part)
-            a, b = np.full(n, x.data_ptr(), dtype=np.uint64), np.array([base + p * step for p in part], dtype=np.uint64)
+            a, b = np.full(n, table[0], dtype=np.uint64), np.array([base + p * step for p in part], dtype=np.uint64)
             la, lb = np.full(n, l, dtype=np.uint32), np.full(n, cache._limbs, dtype=np.uint32)
             nbytes = int(LIB.b2_multiply_relin_batch_workspace_bytes(ctx._h, l, n))
             ws, out = torch.empty(nbytes // 8, dtype=torch.int64, device=ctx.device), ctx.empty(n, 2, l - 1)
@@ -308,11 +309,11 @@ def cached_score_times_v(context, relin_key, galois_key, scores, cache, pages, m
         raise ValueError("score_times_v: positions_per_ct must be a power of 2")
     if cache.ctx is not ctx:
         raise ValueError("ciphertext_cache: the cache belongs to another context")
-    first = scores[0]
-    for s in scores:
-        _check_plain(s, mask_pt)
-        if s._size != 2 or s._chain_index != first._chain_index or abs(s._scale - first._scale) > 1e-9 * first._scale:
-            raise ValueError("score_times_v: scores of one level and one scale are wanted")
+    first, _, _ = _operands(ctx, [scores])
+    _check_plain(first, mask_pt)
+    if mask_pt.data.shape != (first._limbs, ctx.N) or mask_pt.data.get_device() != ctx.device:
+        raise ValueError("encrypted and plain parameter mismatch")
+    mask = mask_pt.data.contiguous()
     l, nominal, spread = first._limbs, first._scale, []
     if l < 3:
         raise ValueError("end of modulus switching chain reached")
@@ -320,7 +321,7 @@ def cached_score_times_v(context, relin_key, galois_key, scores, cache, pages, m
         for p0 in range(0, len(scores), BATCH):
             x = torch.stack([s.data for s in scores[p0:p0 + BATCH]])
             n = x.shape[0]
-            check(LIB.b2_ct_op(ctx._h, 2, l, 2 * n, x.data_ptr(), mask_pt.data.data_ptr(), x.data_ptr(), _stream()))
+            check(LIB.b2_ct_op(ctx._h, 2, l, 2 * n, x.data_ptr(), mask.data_ptr(), x.data_ptr(), _stream()))
             m, ws = ctx.empty(n, 2, l - 1), ctx.empty(2 * n)
             check(LIB.b2_rescale_rounded_batch(ctx._h, l, n, x.data_ptr(), m.data_ptr(), ws.data_ptr(), ws.numel() * 8, _stream()))
             b = d_head // 2

@@ -13,14 +13,16 @@ t * heads * d_head + h * d_head + i of a ciphertext holds element i of head h at
 Elements of a head beyond its pairs pass unchanged. Positions that are dropped (`keep`), and slots of no position, come out as zeros:
 a decoding step's one position goes into its place of a page that way, without a mask of its own.
 """
+from array import array
+
 import torch
 
-from . import _rescale_rounded, add, hoist_rotations, multiply_plain, plaintext
+from . import _operands, hoist_rotations, plaintext
 from ._native import LIB, check, current_stream as _stream, on_device
 
 _PACKINGS = {"pairs": 0, "halves": 1, "interleaved": 2}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
-CHUNK = 16  # ciphertexts whose factors are encoded at a time
+CHUNK = 16  # ciphertexts that go through each kernel together
 
 
 class rotary:
@@ -29,7 +31,7 @@ class rotary:
         scaling: a factor on sines and cosines"""
         if packing not in _PACKINGS:
             raise ValueError("rotary: packing is 'pairs', 'halves' or 'interleaved'")
-        f = torch.as_tensor(inv_freq, dtype=torch.float64).reshape(-1).to(device=context.device).contiguous()
+        f = torch.as_tensor(inv_freq, dtype=torch.float64).reshape(-1).to(device=context.device).clone()
         heads, d_head, pairs = int(heads), int(d_head), f.numel()
         if heads < 1 or d_head < 1 or heads * d_head > context.N // 2:
             raise ValueError("rotary: heads * d_head must be in [1, slots]")
@@ -44,6 +46,7 @@ class rotary:
         self.inv_freq, self.axes = f, torch.tensor(a, dtype=torch.int32, device=context.device)
         self.step = pairs if packing == "halves" else 1
         self._vecs = 1 if packing == "pairs" else 3
+        torch.cuda.synchronize(context.device)  # the tables are there for whichever stream comes first
 
     def factors(self, positions, keep=None, conjugate=False):
         """The factors of `positions` ([tokens] or [tokens][axes], int32, int64, float32 or float64, any strides) as complex128
@@ -73,6 +76,8 @@ class rotary:
         ctx = self.ctx
         if factors.dim() != 3 or factors.dtype != torch.complex128 or factors.shape[2] != ctx.N // 2:
             raise ValueError("rotary: factors are complex128 [vectors][ciphertexts][slots]")
+        if encoder.ctx is not ctx:
+            raise ValueError("rotary: the encoder belongs to another context")
         if chain_index < 1:
             raise ValueError("chain index out of range")
         l = ctx.limbs_at(chain_index)
@@ -87,9 +92,8 @@ class rotary:
         vals = factors.to(device=ctx.device).clone(memory_format=torch.contiguous_format)  # overwritten by the transform
         coeffs, data = torch.empty(vecs * n, ctx.N, dtype=torch.int64, device=ctx.device), ctx.empty(vecs, n, l)
         with on_device(ctx):
-            for k, z in enumerate(vals.view(vecs * n, -1)):
-                check(LIB.b2_encode_coeffs(ctx._h, z.data_ptr(), encoder._d_rot.data_ptr(), encoder._d_ksi.data_ptr(), scale / encoder.slots,
-                                           coeffs[k].data_ptr(), _stream()))
+            check(LIB.b2_encode_coeffs_batch(ctx._h, vecs * n, vals.data_ptr(), encoder._d_rot.data_ptr(), encoder._d_ksi.data_ptr(), scale / encoder.slots,
+                                             coeffs.data_ptr(), _stream()))
             check(LIB.b2_expand_single_chain_batch(ctx._h, l, vecs * n, coeffs.data_ptr(), data.data_ptr(), _stream()))
         return [[self._plain(data[v, i], chain_index, l, scale) for i in range(n)] for v in range(vecs)]
 
@@ -99,25 +103,37 @@ class rotary:
         return pt
 
     def apply(self, xs, plaintexts, galois_key=None):
-        """the ciphertexts xs rotated by the encoded factors, one level further down (rounded to nearest), at their scale. "halves" and "interleaved"
-        want a Galois key for the steps +-`step`."""
-        ctx = self.ctx
-        vecs = self._vecs
+        """the ciphertexts xs (of one level and scale) rotated by the encoded factors, one level further down (rounded to nearest), at
+        their scale. "halves" and "interleaved" want Galois keys for the steps +-`step`."""
+        ctx, vecs = self.ctx, self._vecs
         if len(plaintexts) != vecs or any(len(v) != len(xs) for v in plaintexts):
             raise ValueError("rotary: as many encoded factors as ciphertexts are wanted")
-        if vecs == 3 and xs and galois_key is None:
+        if not len(xs):
+            return []
+        if vecs == 3 and galois_key is None:
             raise ValueError("Galois key not present")
+        first, _, _ = _operands(ctx, [xs])
+        l = first._limbs
+        if any(pt._chain_index != first._chain_index or pt.data.shape != (l, ctx.N) or pt.data.get_device() != ctx.device for v in plaintexts for pt in v):
+            raise ValueError("encrypted and plain parameter mismatch")
+        if l < 2:
+            raise ValueError("end of modulus switching chain reached")
         out = []
         with on_device(ctx):
-            for i, x in enumerate(xs):
-                y = multiply_plain(ctx, x, plaintexts[0][i])
-                if vecs == 3:
-                    up, down = hoist_rotations(ctx, x, galois_key, [self.step, -self.step])
-                    y = add(ctx, add(ctx, y, multiply_plain(ctx, up, plaintexts[1][i])), multiply_plain(ctx, down, plaintexts[2][i]))
-                y = _rescale_rounded(ctx, y)
-                y.set_scale(x._scale)
-                out.append(y)
+            for i in range(0, len(xs), CHUNK):
+                out += self._apply(xs[i:i + CHUNK], [v[i:i + CHUNK] for v in plaintexts], galois_key, l)
         return out
+
+    def _apply(self, xs, plaintexts, galois_key, l):
+        ctx, n, first = self.ctx, len(xs), xs[0]
+        terms = [[x] for x in xs] if self._vecs == 1 else [[x] + hoist_rotations(ctx, x, galois_key, [self.step, -self.step]) for x in xs]
+        _, cts, held = _operands(ctx, terms)
+        factors = [pt.data.contiguous() for i in range(n) for pt in (v[i] for v in plaintexts)]
+        pts = array("Q", [t.data_ptr() for t in factors])
+        y, out, ws = ctx.empty(n, 2, l), ctx.empty(n, 2, l - 1), ctx.empty(2 * n)
+        check(LIB.b2_multiply_plain_sum(ctx._h, l, n, self._vecs, cts.buffer_info()[0], pts.buffer_info()[0], y.data_ptr(), _stream()))
+        check(LIB.b2_rescale_rounded_batch(ctx._h, l, n, y.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel() * 8, _stream()))
+        return [first._like(z, chain_index=first._chain_index + 1, scale=x._scale) for x, z in zip(xs, out.unbind(0))]
 
     def forward(self, encoder, xs, positions, keep=None, conjugate=False, galois_key=None):
         """factors, encode and apply for ciphertexts of one level, CHUNK of them at a time"""

@@ -222,6 +222,54 @@ def test_views_that_are_not_contiguous(mixed):
     assert np.array_equal(cache.page(other).numpy(), x[:, :5])
 
 
+def test_words_that_are_not_there(mixed):
+    """ciphertexts on the host, of another type, or with fewer words than their level has never reach a kernel"""
+    rng = np.random.default_rng(18)
+    good = _ct(mixed, _residues(rng, mixed, 2, 4))
+    cache = ph.ciphertext_cache(mixed, good.chain_index(), 2)
+    (page, _) = cache.allocate(2)
+    bad = [good._like(good.data.cpu()), good.clone(), good.clone(), good.clone(), good._like(good.data[:, :3])]
+    bad[1].data = good.data[:1]
+    bad[2].data = good.data.double()
+    bad[3].data = good.data[..., :N // 2]
+    for ct in bad:
+        for call in (lambda: ph.multiply_sum(mixed, [good, ct], [good, good]), lambda: ph.multiply_sum(mixed, [ct], [good]),
+                     lambda: cache.multiply_sum([good, ct], [page, page]), lambda: ph.cached_qkt(mixed, None, None, ct, cache, [page], 2)):
+            with pytest.raises(ValueError):
+                call()
+    for ct in bad[:2] + bad[3:4]:
+        for call in (lambda: cache.store(page, ct), lambda: cache.append(page, ct)):
+            with pytest.raises(ValueError):
+                call()
+    mask = ph.plaintext.from_numpy(mixed, _residues(rng, mixed, 4), good.chain_index())
+    mask.data = mask.data[:3]
+    with pytest.raises(ValueError, match="mismatch"):
+        ph.cached_score_times_v(mixed, None, None, [good], cache, [page], mask, 2, 4, 2)
+
+
+@pytest.mark.parametrize("terms", [1, 2, 3, 4])
+@pytest.mark.parametrize("n", [1, 5, 33, 70])
+def test_sums_of_ciphertexts_times_plaintexts(mixed, n, terms):
+    """what rotary positions are applied with: n sums in one launch (of at most 32), against single products and additions"""
+    rng = np.random.default_rng(n * 10 + terms)
+    cts = [_ct(mixed, _residues(rng, mixed, 2, 8)) for _ in range(7)]
+    pts = [ph.plaintext.from_numpy(mixed, _residues(rng, mixed, 8), 1) for _ in range(5)]
+    pick = [[(int(rng.integers(7)), int(rng.integers(5))) for _ in range(terms)] for _ in range(n)]
+    a = np.array([cts[i].data.data_ptr() for row in pick for i, _ in row], dtype=np.uint64)
+    b = np.array([pts[j].data.data_ptr() for row in pick for _, j in row], dtype=np.uint64)
+    out = mixed.empty(n, 2, 8)
+    check(LIB.b2_multiply_plain_sum(mixed._h, 8, n, terms, a.ctypes.data, b.ctypes.data, out.data_ptr(), stream()))
+    for k in {0, n // 2, n - 1}:
+        want = ph.add_many(mixed, [ph.multiply_plain(mixed, cts[i], pts[j]) for i, j in pick[k]])
+        assert torch.equal(out[k], want.data)
+    for args, match in [((0, terms), "bad argument"), ((n, 0), "terms"), ((n, 5), "terms")]:
+        with pytest.raises(ValueError, match=match):
+            check(LIB.b2_multiply_plain_sum(mixed._h, 8, *args, a.ctypes.data, b.ctypes.data, out.data_ptr(), stream()))
+    a[0] += np.uint64(8)
+    with pytest.raises(ValueError, match="aligned"):
+        check(LIB.b2_multiply_plain_sum(mixed._h, 8, n, terms, a.ctypes.data, b.ctypes.data, out.data_ptr(), stream()))
+
+
 # ---- streams and graphs ---------------------------------------------------------------------------------------------------------
 def test_captured_calls_replay(mixed):
     rng = np.random.default_rng(12)
@@ -373,7 +421,14 @@ def test_what_is_refused(mixed):
                       (dict(src=cache.data.data_ptr() + 32, s=d.ctypes.data), "overlaps"), (dict(src=other.data.data_ptr(), sl=5, s=d.ctypes.data), "level")]:
         with pytest.raises(ValueError, match=match):
             check(LIB.b2_pages_move(*args(**kw)))
+    for kw in (dict(src=cache.data.data_ptr(), sl=7, s=d.ctypes.data), dict(src=cache.data.data_ptr(), limbs=5, s=d.ctypes.data)):
+        with pytest.raises(ValueError, match="another shape"):
+            check(LIB.b2_pages_move(*args(**kw)))
     out = mixed.empty(3, 6)
+    one_page = np.array([cache.data.data_ptr()], dtype=np.uint64)
+    for at in (cache.data.data_ptr(), cache.data.data_ptr() + 8 * (2 * 6 * N - 4), cache.data.data_ptr() - 8 * (3 * 6 * N - 4)):
+        with pytest.raises(ValueError, match="overlaps"):
+            check(LIB.b2_multiply_sum(mixed._h, 6, 1, 1, one_page.ctypes.data, 6, one_page.ctypes.data, 6, at, stream()))
     a = np.array([cache.data.data_ptr(), cache.data.data_ptr() + 8], dtype=np.uint64)
     for n, la, lb, l, match in [(2, 6, 6, 6, "aligned"), (0, 6, 6, 6, "at least"), (1, 5, 6, 6, "below"), (1, 6, 9, 6, "below"), (1, 6, 6, 0, "size_Ql")]:
         with pytest.raises(ValueError, match=match):

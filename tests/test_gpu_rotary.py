@@ -191,6 +191,9 @@ def test_what_is_refused(ctx):
             rot.encode(*args)
     with pytest.raises(ValueError, match="as many"):
         rot.apply([], rot.encode(enc, fac, 1))
+    other = _ctx(13)
+    with pytest.raises(ValueError, match="another context"):
+        rot.encode(ph.ckks_encoder(other), fac, 1)
     with pytest.raises(ValueError, match="scale out of bounds"):
         ph.rotary(ctx, [1.0], 4, 8, scaling=1e9).encode(enc, fac, 1)
     out = torch.empty(4096, dtype=torch.complex128, device="cuda")
@@ -222,6 +225,36 @@ def kit():
 # units where the slot's root zeta is next to 1, and in the second polynomial that times |s(zeta)|, below 4 sqrt(2 N / 3) = 296 for a
 # ternary secret of N = 8192: 1.5e6 units, 1.4e-6. A slot takes one of the two rotations (A and B do not overlap).
 CT_TOL = {"pairs": 1e-7, "halves": 1.5e-6, "interleaved": 1.5e-6}
+
+
+@pytest.mark.parametrize("vectors", [1, 3, 17])
+def test_batch_of_encodings_is_the_single_ones(kit, vectors):
+    ctx, enc = kit["ctx"], kit["enc"]
+    n = ctx.N // 2
+    z = torch.randn(vectors, n, dtype=torch.complex128, device="cuda", generator=torch.Generator("cuda").manual_seed(vectors))
+    one, many = (torch.empty(vectors, ctx.N, dtype=torch.int64, device="cuda") for _ in range(2))
+    for k in range(vectors):
+        check(LIB.b2_encode_coeffs(ctx._h, z[k].clone().data_ptr(), enc._d_rot.data_ptr(), enc._d_ksi.data_ptr(), 2.0 ** 30 / n, one[k].data_ptr(), stream()))
+    check(LIB.b2_encode_coeffs_batch(ctx._h, vectors, z.data_ptr(), enc._d_rot.data_ptr(), enc._d_ksi.data_ptr(), 2.0 ** 30 / n, many.data_ptr(), stream()))
+    assert torch.equal(one, many) and bool(one.any())
+    with pytest.raises(ValueError, match="bad argument"):
+        check(LIB.b2_encode_coeffs_batch(ctx._h, 0, z.data_ptr(), enc._d_rot.data_ptr(), enc._d_ksi.data_ptr(), 1.0, many.data_ptr(), stream()))
+
+
+def test_more_ciphertexts_than_go_together(kit):
+    """the ciphertexts of a long prompt, 16 at a time, are each what they are alone"""
+    ctx, enc, sk = kit["ctx"], kit["enc"], kit["sk"]
+    rot = ph.rotary(ctx, [1.0, 0.1], 64, 16, packing="interleaved")
+    n = 19
+    x = sk.encrypt_symmetric(ctx, enc.encode_double_vector(ctx, np.random.default_rng(1).uniform(-1, 1, ctx.N // 2), 2.0 ** 40, 3))
+    pos = torch.arange(n * rot.positions_per_ct - 1, device="cuda")
+    out = rot.forward(enc, [x] * n, pos, galois_key=kit["glk"])
+    assert len(out) == n
+    for i in (0, 15, 16, n - 1):
+        per = rot.positions_per_ct
+        (alone,) = rot.forward(enc, [x], pos[i * per:(i + 1) * per], galois_key=kit["glk"])
+        assert torch.equal(alone.data, out[i].data)
+    assert rot.forward(enc, [], pos[:0], galois_key=kit["glk"]) == []
 
 
 @pytest.mark.parametrize("packing,d_head,pairs", [("pairs", 8, 8), ("pairs", 12, 5), ("halves", 16, 8), ("halves", 20, 8), ("interleaved", 16, 8), ("interleaved", 10, 4)])
@@ -257,6 +290,10 @@ def test_rotated_ciphertexts(kit, packing, d_head, pairs):
             rot.forward(enc, cts, pos)
     with pytest.raises(ValueError, match="positions for"):
         rot.forward(enc, cts[:1], pos, galois_key=glk)
+    with pytest.raises(ValueError, match="mismatch"):  # factors of another level
+        rot.apply(cts, rot.encode(enc, rot.factors(pos), 1), glk)
+    with pytest.raises(ValueError, match="mismatch"):  # ciphertexts of two levels
+        rot.forward(enc, [cts[0], ph.mod_switch_to_next(ctx, cts[1])], pos, galois_key=glk)
     out = rot.forward(enc, cts, pos, galois_key=glk)
     for i, ct in enumerate(out):
         assert ct.chain_index() == 3 and ct.scale() == 2.0 ** 40
