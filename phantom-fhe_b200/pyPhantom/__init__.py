@@ -585,28 +585,29 @@ def multiply_sum(ctx, a, b):
 def _operands(ctx, rows):
     """(the first ciphertext, the addresses of all as an array, copies of strided ones, which live until the launch)"""
     first = rows[0][0]
-    chain_index, limbs, scale, N, device = first._chain_index, first._limbs, first._scale, ctx.N, ctx.device
-    if chain_index < 1 or limbs != ctx.limbs_at(chain_index):
+    l, N, device, int64 = first._limbs, ctx.N, ctx.device, torch.int64
+    if first._chain_index < 1 or l != ctx.limbs_at(first._chain_index):
         raise ValueError("encrypted1 and encrypted2 parameter mismatch")
-    addresses, held = array("Q"), []
+    kind, scale, words = (first._chain_index, l, N, True, 2), first._scale, 2 * l * N
+    addresses, held = [], []
     for row in rows:
         for ct in row:
-            if ct._chain_index != chain_index or ct._limbs != limbs or ct._N != N:
+            if (ct._chain_index, ct._limbs, ct._N, ct._is_ntt_form, ct._size) != kind:
+                if not ct._is_ntt_form:
+                    raise ValueError("encrypted1 and encrypted2 must be in NTT form")
+                if ct._size != 2:
+                    raise ValueError("only 2-polynomial operands are built")
                 raise ValueError("encrypted1 and encrypted2 parameter mismatch")
-            if not ct._is_ntt_form:
-                raise ValueError("encrypted1 and encrypted2 must be in NTT form")
-            if ct._size != 2:
-                raise ValueError("only 2-polynomial operands are built")
             if ct._scale != scale and not _are_close(ct._scale, scale):
                 raise ValueError("scale mismatch")
             data = ct.data
-            if data.numel() != 2 * limbs * N or data.dtype != torch.int64 or data.get_device() != device:
+            if data.numel() != words or data.dtype is not int64 or data.get_device() != device:
                 raise ValueError("the ciphertext's words are not on the context's device, or not as many as its level has")
             if not data.is_contiguous():
                 data = data.contiguous()
                 held.append(data)
             addresses.append(data.data_ptr())
-    return first, addresses, held
+    return first, array("Q", addresses), held
 
 
 def _multiply_sum(ctx, a, table, b_limbs, b_chain_index, b_scale):

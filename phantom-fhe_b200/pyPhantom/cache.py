@@ -12,6 +12,7 @@ replays the moves of the numbers it was captured with.
 """
 import heapq
 from array import array
+from operator import index
 
 import numpy as np
 import torch
@@ -54,15 +55,14 @@ class ciphertext_cache:
         return self._held[self._number(page)]
 
     def _number(self, page):
-        page = int(page)
+        page = index(page)
         if not 0 <= page < len(self._held):
             raise ValueError("ciphertext_cache: page out of range")
         return page
 
     def _live(self, pages):
-        """the page numbers as a list, each of an allocated page"""
-        if type(pages) is not list:
-            pages = [int(p) for p in pages]
+        """the page numbers as a list of integers, each of an allocated page"""
+        pages = list(map(index, pages))
         held = self._held
         try:
             ok = not pages or (min(pages) >= 0 and all(map(held.__getitem__, pages)))

@@ -92,6 +92,13 @@ def test_page_numbers_of_any_kind(new):
     assert _marks(cache, range(6)) == [3, 4, 3, 4, 3, 4]
     cache.free(np.array([5]))
     assert cache.free_pages() == 1 and cache.allocate(1) == [5]
+    pages = list(torch.tensor([4, 4]))  # two objects, one page
+    with pytest.raises(ValueError, match="more often"):
+        cache.free(pages)
+    assert cache.fork(pages, tail=0) == [[4, 4]] and cache.held(4) == 3
+    assert cache.compact([pages, [np.int64(1)]]) == [[0, 0], [1]]
+    with pytest.raises(TypeError):
+        cache.free([0.0])
 
 
 @pytest.mark.parametrize("call,match", [

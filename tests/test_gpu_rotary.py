@@ -203,7 +203,7 @@ def test_what_is_refused(ctx):
                                     out, stream()))
 
     for kw, match in [(dict(packing=3), "packing"), (dict(kind=4), "type"), (dict(heads=1 << 40, d_head=1 << 40), "slots"), (dict(heads=257), "slots"),
-                      (dict(pairs=0), "pairs"), (dict(pairs=9), "pairs"), (dict(pairs=5, packing=2), "pairs"), (dict(pos=0), "null"), (dict(out=out.data_ptr() + 8), "aligned"),
+                      (dict(pairs=0), "pairs"), (dict(pairs=9), "pairs"), (dict(pairs=5, packing=2), "pairs"), (dict(pos=0), "null"), (dict(out=out.data_ptr() + 8), "aligned"), (dict(pos=p.data_ptr() + 4), "aligned"),
                       (dict(tokens=1 << 40), "2\\^30")]:
         with pytest.raises(ValueError, match=match):
             c_entry(**kw)
