@@ -513,6 +513,101 @@ def test_attention_products_over_pages(kit, pages):
             call()
 
 
+@pytest.mark.parametrize("log_n,chain,special,bconv", [(12, 4, 1, None), (13, 5, 1, None), (13, 5, 3, "int"), (14, 4, 2, None), (15, 6, 2, "fp"), (16, 5, 2, None), (17, 4, 1, None)])
+def test_attention_products_in_every_ring(log_n, chain, special, bconv, monkeypatch):
+    """down to the last level the products have room for, in every ring, with and without the batched key switch, against numbers and
+    against the lists' forms; a page named twice counts twice"""
+    n, slots = 1 << log_n, 1 << (log_n - 1)
+    if bconv:
+        monkeypatch.setenv("B2_BCONV", bconv)
+    heads, d_head = 4, 8
+    d_total, per = 32, slots // 32
+    steps = {1, 2, 4, -1, -2, -4} | {32 << k for k in range(log_n - 6)}
+    parms = ph.params(ph.scheme_type.ckks)
+    parms.set_poly_modulus_degree(n)
+    parms.set_coeff_modulus(ph.create_coeff_modulus(n, [60] + [40] * (chain - 1) + [60] * special))
+    parms.set_special_modulus_size(special)
+    parms.set_galois_elts(sorted(ph.get_elts_from_steps(sorted(steps), n)))
+    ctx = ph.context(parms)
+    sk, enc = ph.secret_key(ctx, seed=log_n), ph.ckks_encoder(ctx)
+    rlk, glk = sk.gen_relinkey(ctx), sk.create_galois_keys(ctx)
+    rng = np.random.default_rng(log_n)
+    top = ctx.size_Q - 3  # four limbs left: q * k, the mask and score x V take three
+    encrypt = lambda v: sk.encrypt_symmetric(ctx, enc.encode_double_vector(ctx, v, SCALE, top))
+    decrypt = lambda ct: np.asarray(enc.decode_complex_vector(ctx, sk.decrypt(ctx, ct))).real
+    q = rng.uniform(-1, 1, (heads, d_head))
+    K, V = rng.uniform(-1, 1, (2, 3, per, heads, d_head))
+    cache = ph.ciphertext_cache(ctx, top, 3, 2, scale=SCALE)
+    for p in cache.allocate(3):
+        cache.store(p, encrypt(K[p].ravel()))
+        cache.store(p, encrypt(V[p].ravel()), plane=1)
+    cq, table = encrypt(np.tile(q.ravel(), per)), [2, 0, 2, 1]
+    scores = ph.cached_qkt(ctx, rlk, glk, cq, cache, table, d_head)
+    lists = ph.compute_qkt(ctx, rlk, glk, cq, cache.ciphertexts(table), d_head)
+    mask = np.zeros((per, heads, d_head))
+    mask[:, :, 0] = 1.0
+    mask_pt = enc.encode_double_vector(ctx, mask.ravel(), float(ctx.primes[ctx.limbs_at(top + 1) - 1]), top + 1)
+    out = ph.cached_score_times_v(ctx, rlk, glk, scores, cache, table, mask_pt, d_head, d_total, per, plane=1)
+    plain = ph.score_times_v(ctx, rlk, glk, lists, cache.ciphertexts(table, plane=1), mask_pt, d_head, d_total, per)
+    assert out.chain_index() == plain.chain_index() == ctx.size_Q and out.data.shape == plain.data.shape == (2, 1, n)
+    # ModDown's floor as above, 2 N / pi * |s| * (1 + (alpha - 1) / 2) units of 2^-40 in the slots next to 1, |s| < 4 sqrt(2 N / 3): a
+    # score takes it (2 d_head - 1) times over, a value d_head + 3 times more, over the slots near 1 (sum 1/j < 12); and the rescales
+    # of the lists' forms floor, which adds half a unit to each of theirs
+    unit = 2 * n / np.pi * 4 * np.sqrt(2 * n / 3) * (1.5 + (special - 1) / 2) * 2.0 ** -40
+    score_tol, value_tol = (2 * d_head - 1) * unit, 12 * (3 * d_head + 2) * unit
+    want = np.einsum("hi,cthi->cth", q, K[table])
+    for i in range(4):
+        for ct in (scores[i], lists[i]):
+            assert np.max(np.abs(decrypt(ct).reshape(per, heads, d_head)[:, :, 0] - want[i])) < score_tol
+    total = np.einsum("cth,cthi->hi", want, V[table]).ravel()
+    for ct in (out, plain):
+        got = decrypt(ct)
+        assert np.max(np.abs(got[:d_total] - total)) < value_tol and np.max(np.abs(got[-d_total:] - total)) < value_tol
+
+
+def test_a_captured_decoding_step(kit):
+    """rotation of the query, its products with the cached keys and values, and a fork of the pages in one graph: replayed, it gives
+    what the calls give, for whatever the query and the pages then hold"""
+    ctx, enc, rlk, glk = kit["ctx"], kit["enc"], kit["rlk"], kit["glk"]
+    rng = np.random.default_rng(19)
+    rot = ph.rotary(ctx, [1.0, 0.01], HEADS, D_HEAD, packing="halves")
+    cache = ph.ciphertext_cache(ctx, 2, 6, 2, scale=SCALE)
+    table = cache.allocate(2)
+    fresh = lambda: _enc(kit, rng.uniform(-1, 1, SLOTS), 1)
+    low = lambda: _enc(kit, rng.uniform(-1, 1, SLOTS), 2)
+    mask = np.zeros((PER, HEADS, D_HEAD))
+    mask[:, :, 0] = 1.0
+    mask_pt = enc.encode_double_vector(ctx, mask.ravel(), float(ctx.primes[ctx.limbs_at(3) - 1]), 3)
+    for p in table:
+        cache.store(p, low()), cache.store(p, low(), plane=1)
+    q, pos = fresh(), torch.full((PER,), 3, device="cuda")
+    copy = cache.allocate(2)
+
+    def step():
+        (r,) = rot.forward(enc, [q], pos, galois_key=glk)
+        cache.copy(copy, table)
+        scores = ph.cached_qkt(ctx, rlk, glk, r, cache, copy, D_HEAD)
+        return ph.cached_score_times_v(ctx, rlk, glk, scores, cache, copy, mask_pt, D_HEAD, D_TOTAL, PER, plane=1)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for k in range(3):
+        q.data.copy_(fresh().data)
+        pos.fill_(100 * k)
+        cache.store(table[k % 2], low(), plane=k % 2)
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.data.clone()
+        cache.data[:, copy] = 0
+        assert torch.equal(step().data, got) and bool(got.any())
+
+
 @pytest.mark.parametrize("packing", ["halves", "interleaved"])
 def test_generation_step(kit, packing):
     """keys and values of a few positions rotated and put into pages one after another, the sequence forked, one more position in
