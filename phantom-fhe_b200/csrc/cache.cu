@@ -14,16 +14,14 @@ namespace b2 {
 // Bound by HBM: a copy's rate, half reads and half writes. Four steps a batch keep the registers at 64, so that an SM has 1024
 // threads with 128 bytes each in flight; with eight (126 registers, 512 threads) 47 pages of 2 MB in four planes change places in
 // 159 us, with four in 124 (6.36 TB/s), with two in 130.
-template <int CAP>
-struct PageMoves {
+struct PageMoves {  // 4 KB of parameters: they cost a launch less than 0.1 us over 256 bytes
     PageArgs a;
     uint16_t end[PAGE_LANES];
-    PageStep step[CAP];
+    PageStep step[PAGE_STEPS];
 };
 constexpr int PAGE_BATCH = 4;
 
-template <int CAP>
-__global__ void __launch_bounds__(256, 4) pages_move_kernel(const __grid_constant__ PageMoves<CAP> m) {
+__global__ void __launch_bounds__(256, 4) pages_move_kernel(const __grid_constant__ PageMoves m) {
     pdl_enter();
     const PageArgs &a = m.a;
     const uint32_t lane = blockIdx.y, c0 = (blockIdx.x * 256 + threadIdx.x) * 4;
@@ -56,19 +54,13 @@ __global__ void __launch_bounds__(256, 4) pages_move_kernel(const __grid_constan
     }
 }
 
-template <int CAP>
-static void move_pages(const PageArgs &a, const PageStep *steps, const uint32_t *ends, uint32_t lanes, uint32_t planes, cudaStream_t s) {
-    PageMoves<CAP> m;
+void launch_pages_move(const PageArgs &a, const PageStep *steps, const uint32_t *ends, uint32_t lanes, uint32_t planes, cudaStream_t s) {
+    PageMoves m;
     m.a = a;
     for (uint32_t i = 0; i < lanes; i++) m.end[i] = (uint16_t)ends[i];
     std::copy_n(steps, ends[lanes - 1], m.step);
     // 32-byte columns of a page: half / 2, a multiple of 2048
-    launch_k(pages_move_kernel<CAP>, dim3(a.half / 512, lanes, planes), 256, 0, s, m);
-}
-
-void launch_pages_move(const PageArgs &a, const PageStep *steps, const uint32_t *ends, uint32_t lanes, uint32_t planes, cudaStream_t s) {
-    if (ends[lanes - 1] <= PAGE_STEPS_FEW) move_pages<PAGE_STEPS_FEW>(a, steps, ends, lanes, planes, s);
-    else move_pages<PAGE_STEPS>(a, steps, ends, lanes, planes, s);
+    launch_k(pages_move_kernel, dim3(a.half / 512, lanes, planes), 256, 0, s, m);
 }
 
 // ---- sum of products of ciphertexts ------------------------------------------------------------------------------------

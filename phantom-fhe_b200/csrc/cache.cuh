@@ -10,7 +10,7 @@
 namespace b2 {
 
 // ---- pages: [plane][page][2][limbs][N] --------------------------------------------------------------------------------
-constexpr int PAGE_STEPS = 480, PAGE_STEPS_FEW = 14, PAGE_LANES = 64;
+constexpr int PAGE_STEPS = 480, PAGE_LANES = 64;
 struct PageArgs {
     uint64_t *pool;
     const uint64_t *src;            // the pool itself, or another one at the same level or a higher one
