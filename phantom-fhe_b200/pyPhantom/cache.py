@@ -165,6 +165,8 @@ class ciphertext_cache:
         other = self if source is None else source
         if other.ctx is not self.ctx or other._planes != self._planes or other._limbs < self._limbs:
             raise ValueError("ciphertext_cache: the source has another context, other planes or a lower level")
+        if abs(other._scale - self._scale) > 1e-9 * self._scale:
+            raise ValueError("scale mismatch")
         dst = self._live(dst)
         if any(self._held[p] > 1 for p in dst):
             raise ValueError("ciphertext_cache: the page is shared (fork the table first)")
@@ -206,9 +208,11 @@ class ciphertext_cache:
         (page,) = self._live([page])
         if self._held[page] > 1:
             raise ValueError("ciphertext_cache: the page is shared (fork the table first)")
-        if ct._size != 2 or not ct._is_ntt_form or ct.data.shape != (2, ct._limbs, self.ctx.N) or ct.data.get_device() != self.ctx.device:
+        data = ct.data
+        if (ct._size != 2 or not ct._is_ntt_form or data.shape != (2, ct._limbs, self.ctx.N) or data.dtype != torch.int64
+                or data.get_device() != self.ctx.device):
             raise ValueError("ciphertext_cache: a two-polynomial ciphertext in NTT form on the context's device is wanted")
-        if ct._chain_index > self._chain_index:
+        if ct._chain_index > self._chain_index or ct._limbs < self._limbs:
             raise ValueError("cannot switch to higher level modulus")
         if abs(ct._scale - self._scale) > 1e-9 * self._scale:
             raise ValueError("scale mismatch")

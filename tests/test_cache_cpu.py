@@ -37,6 +37,12 @@ def _marks(cache, table):
     return [int(cache.data[0, p, 0, 0, 0]) for p in table]
 
 
+def _scaled(cache):
+    other = ph.ciphertext_cache(cache.ctx, 1, 2, 2, scale=2.0 ** 39)
+    other.allocate(2)
+    return other
+
+
 def _mark(cache, page, value):
     cache.data[:, page] = value
 
@@ -113,6 +119,10 @@ def test_page_numbers_of_any_kind(new):
     (lambda c, o: c.multiply_sum([c.page(0)], [5]), "not allocated"), (lambda c, o: c.append(1, c.page(0)), "shared"), (lambda c, o: c.store(1, c.page(0)), "shared"),
     (lambda c, o: c.store(0, o.page(0)), "higher level"), (lambda c, o: c.append(0, c.page(2)._like(c.page(2).data, scale=3.0)), "scale"),
     (lambda c, o: c.append(0, c.page(2)._like(c.page(2).data[:1])), "two-polynomial"),
+    (lambda c, o: c.append(0, c.page(2)._like(c.page(2).data.double())), "two-polynomial"),
+    (lambda c, o: c.append(0, c.page(2)._like(c.page(2).data[:, :2])), "higher level"),  # two limbs that pass for four
+    (lambda c, o: c.store(0, c.page(2)._like(c.page(2).data[:, :2])), "higher level"),
+    (lambda c, o: c.copy([0], [0], source=_scaled(c)), "scale"),
     (lambda c, o: c.multiply_sum([c.page(0)._like(c.page(0).data[:, :2], chain_index=1)], [0]), "parameter mismatch"),
 ])
 def test_refused_calls_change_nothing(new, call, match):
