@@ -71,9 +71,11 @@ void launch_pages_move(const PageArgs &a, const PageStep *steps, const uint32_t 
 // Bound by HBM: 2 (G + 1) limbs a term for 4 G products. One word a thread and load keeps the sums of all arithmetics in 80 registers
 // (G = 1; 768 threads an SM with eight loads each in flight): 32 terms at N = 2^16, 16 limbs of 40 bits take 160.6 us (1.10 GB, 6.84
 // TB/s; 8.6 us for 17 terms of 6 limbs at 2^14), with two words a thread 168 to 193, with U = 8 and 128 registers 159.1, but 177.9
-// against 168.4 on primes of 55 bits. Four queries (24 pages at 2^15, 12 limbs, 0.79 GB): 129.9 us; 181 with each query's sums in
-// 21-bit pieces (72 registers of sums; FP64 products need 24 and take 131 to 137), and on integer primes, whose sums of 30-bit
-// pieces are wide too, the queries go two by two over the same pages: 186.2 against 187 to 259 at once. Terms dealt to four groups of
+// against 168.4 on primes of 55 bits. Four queries (24 pages at 2^15, 12 limbs, 0.79 GB): 128.5 us, 133.7 after two seconds of it, at
+// the 1770 MHz that the power cap leaves (130.5 and 136.5 with the sums brought back every fourth term); 181 with each query's sums in
+// 21-bit pieces (72 registers of sums; FP64 products need 24), and on integer primes, whose sums of 30-bit pieces are wide too, the
+// queries go two by two over the same pages: 186.2 against 187 to 259 at once. Four terms of four queries at a time (168 registers,
+// 12 warps an SM): 127.0, but 193.9 on primes of 55 bits. Terms dealt to four groups of
 // threads that join in shared memory gain 1.3 us of 10 at 60 terms and 96 CTAs and lose everywhere else: not built.
 constexpr int SUM_T = 128;
 template <class S, int G, int U>
@@ -135,12 +137,20 @@ __device__ __forceinline__ void multiply_sum_body(const SumArgs &a, const Mod &m
         }
 }
 
+// FP64 products of primes below 2^41: 2048 of them stay below 2^53, so that no sum of a launch is brought back on the way
+struct SumFpLong : SumFp {
+    static constexpr int FLUSH = 2048;
+};
+static_assert(2 * SUM_TERMS <= SumFpLong::FLUSH);
+
 template <int G, int U, int MIN_CTAS>
 __global__ void __launch_bounds__(SUM_T, MIN_CTAS) multiply_sum_kernel(const __grid_constant__ SumArgs a) {
     pdl_enter();
     const Mod md = a.mod[blockIdx.y];
     if constexpr (G <= 2) {
         with_sum(md.q, [&](auto s) { multiply_sum_body<decltype(s), G, U>(a, md, 0); });
+    } else if (md.q < FP_SMALL_LIMIT) {
+        multiply_sum_body<SumFpLong, G, U>(a, md, 0);
     } else if (md.q < FP_LIMIT) {
         multiply_sum_body<SumFp, G, U>(a, md, 0);
     } else {
