@@ -2635,9 +2635,10 @@ extern "C" int b2_ct_lincomb(b2_ctx *c, size_t l, size_t n_poly, size_t n_terms,
 // ------------------------------------------------------------------------------------------------
 // operators of generation with an encrypted model (cache.cuh)
 // ------------------------------------------------------------------------------------------------
-// How many lanes (blockIdx.y) a launch of page moves is spread over: enough that the grid fills the GPU's resident threads twice,
-// and lanes of about eight moves where there are that many (24 moves of 4.7 MB pages in two planes: 71.9 us in one lane or two,
-// 70.5 in eight of three; eight moves of one source stay together, as a lane reads it once a batch: 49.5 us, 51.5 in four lanes).
+// How many lanes (blockIdx.y) a launch of page moves is spread over: enough that the grid fills the GPU's resident threads twice
+// (90 moves of 0.2 MB pages in six planes: 67.5 us in one lane, 45 in two, 37 in four or more), and lanes of about eight moves where
+// there are that many (24 moves of 4.7 MB pages in two planes: 72 us in lanes of 24, 12 or 6, 74 of three, 82 of one; eight moves of one
+// source, which a lane reads once a batch: 49.6 us together, 52 in two or four lanes, 68 in eight).
 static uint32_t page_lanes(const b2_ctx *c, size_t limbs, size_t planes, size_t moves) {
     const size_t ctas = limbs * c->N / 512 * planes, want = (size_t)c->sm_count * 8;  // of 256 threads with 32 bytes a page each
     return (uint32_t)std::min({std::max((want + ctas - 1) / ctas, moves / 8), moves, (size_t)PAGE_LANES});

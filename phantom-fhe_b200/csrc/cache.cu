@@ -11,9 +11,9 @@ namespace b2 {
 // A thread owns the same 32 bytes of every page and walks its lane's steps, so that moves of a pool onto itself need no second
 // buffer and no order between threads. Loads of a batch of steps go out before its stores: no step reads what an earlier step of
 // the plan wrote, whichever is issued first. Steps of one source that follow one another read it once.
-// Bound by HBM: a copy's rate, half reads and half writes. Four steps a batch keep the registers at 64, so that an SM has 1024
-// threads with 128 bytes each in flight; with eight (126 registers, 512 threads) 47 pages of 2 MB in four planes change places in
-// 159 us, with four in 124 (6.36 TB/s), with two in 130.
+// Bound by HBM: a copy's rate, half reads and half writes. Four steps a batch take 56 registers, so that an SM has 1024 threads with
+// 128 bytes each in flight: 47 pages of 2 MB in four planes change places in 121 us (6.5 TB/s); with eight steps (126 registers, 512
+// threads) in 159, with two in 130.
 struct PageMoves {  // 4 KB of parameters: they cost a launch less than 0.1 us over 256 bytes
     PageArgs a;
     uint16_t end[PAGE_LANES];
@@ -69,8 +69,8 @@ void launch_pages_move(const PageArgs &a, const PageStep *steps, const uint32_t 
 // first is multiplied; sums stay in registers as the prime's arithmetic likes them (sums.cuh) and are reduced once at the end.
 // G queries share one read of the pages.
 // Bound by HBM: 2 (G + 1) limbs a term for 4 G products. One word a thread and load keeps the sums of all arithmetics in 80 registers
-// (G = 1; 768 threads an SM with eight loads each in flight): 32 terms at N = 2^16, 16 limbs of 40 bits take 160.6 us (1.10 GB, 6.84
-// TB/s; 8.6 us for 17 terms of 6 limbs at 2^14), with two words a thread 168 to 193, with U = 8 and 128 registers 159.1, but 177.9
+// (G = 1; 768 threads an SM with sixteen loads each in flight): 32 terms at N = 2^16, 16 limbs of 40 bits take 160.6 us (1.10 GB, 6.84
+// TB/s), 17 terms of 6 limbs at 2^14 11.3 (8.6 out of L2), with two words a thread 168 to 193, with U = 8 and 128 registers 159.1, but 177.9
 // against 168.4 on primes of 55 bits. Four queries (24 pages at 2^15, 12 limbs, 0.79 GB): 128.5 us, 133.7 after two seconds of it, at
 // the 1770 MHz that the power cap leaves (130.5 and 136.5 with the sums brought back every fourth term); 181 with each query's sums in
 // 21-bit pieces (72 registers of sums; FP64 products need 24), and on integer primes, whose sums of 30-bit pieces are wide too, the

@@ -497,6 +497,7 @@ def test_attention_products_over_pages(kit, pages):
     assert launched["multiply_sum"] == 1 and out.chain_index() == 4 and out.scale() == SCALE
     got, want = _dec(kit, out).real, np.einsum("cth,cthi->hi", want_s, V).ravel()
     assert np.max(np.abs(got[:D_TOTAL] - want)) < VALUE_TOL * pages and np.max(np.abs(got[-D_TOTAL:] - want)) < VALUE_TOL * pages
+    assert ph.cached_qkt(ctx, rlk, glk, cq, cache, [], D_HEAD) == [] and cache.ciphertexts([]) == []
     if pages == 3:  # the list forms take the pages as they are, and agree
         lists = ph.compute_qkt(ctx, rlk, glk, cq, cache.ciphertexts(table), D_HEAD)
         assert np.max(np.abs(_dec(kit, lists[1]) - _dec(kit, scores[1]))) < SCORE_TOL
