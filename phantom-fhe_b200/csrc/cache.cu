@@ -68,20 +68,64 @@ void launch_pages_move(const PageArgs &a, const PageStep *steps, const uint32_t 
 // summed before any of them is relinearised. A thread owns one position of a limb and walks the terms, U of them loaded before the
 // first is multiplied; sums stay in registers as the prime's arithmetic likes them (sums.cuh) and are reduced once at the end.
 // G queries share one read of the pages.
-// Bound by HBM: 2 (G + 1) limbs a term for 4 G products. One word a thread and load keeps the sums of all arithmetics in 80 registers
+// Bound by HBM: 2 (G + 1) limbs a term for 3 G products. One word a thread and load keeps the sums of all arithmetics in 80 registers
 // (G = 1; 768 threads an SM with sixteen loads each in flight): 32 terms at N = 2^16, 16 limbs of 40 bits take 160.6 us (1.10 GB, 6.84
-// TB/s), 17 terms of 6 limbs at 2^14 11.3 (8.6 out of L2), with two words a thread 168 to 193, with U = 8 and 128 registers 159.1, but 177.9
-// against 168.4 on primes of 55 bits. Four queries (24 pages at 2^15, 12 limbs, 0.79 GB): 128.5 us, 133.7 after two seconds of it, at
-// the 1770 MHz that the power cap leaves (130.5 and 136.5 with the sums brought back every fourth term); 181 with each query's sums in
-// 21-bit pieces (72 registers of sums; FP64 products need 24), and on integer primes, whose sums of 30-bit pieces are wide too, the
-// queries go two by two over the same pages: 186.2 against 187 to 259 at once. Four terms of four queries at a time (168 registers,
-// 12 warps an SM): 127.0, but 193.9 on primes of 55 bits. Terms dealt to four groups of
-// threads that join in shared memory gain 1.3 us of 10 at 60 terms and 96 CTAs and lose everywhere else: not built.
+// TB/s), 17 terms of 6 limbs at 2^14 11.3 (8.6 out of L2), with two words a thread 168 to 193. More queries take 128 registers and as many
+// terms at a time as those hold: two (24 pages at 2^15, 12 limbs, 0.47 GB) 76.6 us with five terms, 77.4 with four, 80.5 with three;
+// three (0.63 GB) 99.8 with four, 117 with three; four (0.79 GB) 126.8 with three, 129.3 with two. Four queries are where the power cap
+// is felt: after two seconds of them 136.7 us (141.3 with four products a term in place of three). Sums of three and four queries are
+// FP64 products: in 21-bit pieces, 72 registers of sums for four, 181 us; on integer primes, whose sums of 30-bit pieces are as wide, the
+// queries go two by two over the same pages (55 bits: four 182 us; 187 to 259 at once). Terms dealt to four groups of threads that join
+// in shared memory gain 1.3 us of 10 at 60 terms and 96 CTAs and lose everywhere else: not built.
 constexpr int SUM_T = 128;
+
+// FP64 products of primes below 2^41: 2048 of them stay below 2^53, so that no sum of a launch is brought back on the way
+struct SumFpLong : SumFp {
+    static constexpr int FLUSH = 2048;
+};
+static_assert(2 * SUM_TERMS <= SumFpLong::FLUSH);
+
+// The middle sum takes (a0 + a1)(b0 + b1) and loses the two others at the end: three products a term instead of four.
+//   both_a, both_b   the sum of two operands as an operand of S;  TERMS  how many terms the three sums take before they are brought back
+// 21-bit pieces are added piece by piece (22 bits and 21: a term adds 2^44 to the two lower sums, sixty of them stay below 2^50); of
+// FP64 residues below 2^50 one factor may be 2 q, the other is brought below q, and a product is below q; integers are reduced.
+template <class S>
+struct Pair {
+    static constexpr int TERMS = S::FLUSH;
+    __device__ __forceinline__ static typename S::A both_a(uint64_t x, uint64_t y, const typename S::A &, const typename S::A &, const Mod &md, const typename S::K &k) {
+        return S::ld_a(add_mod(x, y, md.q), k);
+    }
+    __device__ __forceinline__ static typename S::B both_b(uint64_t x, uint64_t y, const typename S::B &, const typename S::B &, const Mod &md, const typename S::K &k) {
+        return S::ld_b(add_mod(x, y, md.q), k);
+    }
+};
+template <>
+struct Pair<SumFp21> {
+    using S = SumFp21;
+    static constexpr int TERMS = 60;
+    __device__ __forceinline__ static S::A both_a(uint64_t, uint64_t, const S::A &x, const S::A &y, const Mod &, const S::K &) {
+        return S::A{__dadd_rn(x.l, y.l), __dadd_rn(x.h, y.h)};
+    }
+    __device__ __forceinline__ static S::B both_b(uint64_t, uint64_t, const S::B &x, const S::B &y, const Mod &, const S::K &) {
+        return S::B{__dadd_rn(x.l, y.l), __dadd_rn(x.h, y.h)};
+    }
+};
+template <class F>
+struct PairFp {
+    static constexpr int TERMS = F::FLUSH - 1;
+    __device__ __forceinline__ static SumFp::A both_a(uint64_t x, uint64_t y, const SumFp::A &, const SumFp::A &, const Mod &md, const SumFp::K &k) {
+        return SumFp::ld_a(add_mod(x, y, md.q), k);
+    }
+    __device__ __forceinline__ static SumFp::B both_b(uint64_t, uint64_t, const SumFp::B &x, const SumFp::B &y, const Mod &, const SumFp::K &) { return __dadd_rn(x, y); }
+};
+template <>
+struct Pair<SumFp> : PairFp<SumFp> {};
+template <>
+struct Pair<SumFpLong> : PairFp<SumFpLong> {};
+
 template <class S, int G, int U>
 __device__ __forceinline__ void multiply_sum_body(const SumArgs &a, const Mod &md, uint32_t g0) {
-    constexpr int FULL = S::FLUSH / 2;  // terms that fill a sum: the middle one takes two products of each
-    static_assert(U <= FULL);
+    static_assert(U <= Pair<S>::TERMS);
     const typename S::K k = S::make(md);
     const size_t N = (size_t)1 << a.logN;
     const size_t o = (size_t)blockIdx.y * N + blockIdx.x * SUM_T + threadIdx.x, ga = (size_t)a.la * N, gb = (size_t)a.lb * N;
@@ -104,7 +148,7 @@ __device__ __forceinline__ void multiply_sum_body(const SumArgs &a, const Mod &m
                 }
             }
         }
-        if (pending + U > FULL) {
+        if (pending + U > Pair<S>::TERMS) {
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll
@@ -115,33 +159,30 @@ __device__ __forceinline__ void multiply_sum_body(const SumArgs &a, const Mod &m
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (t + u < a.terms) {
-                const typename S::A y0 = S::ld_a(b0[u], k), y1 = S::ld_a(b1[u], k);
+                const typename S::A y0 = S::ld_a(b0[u], k), y1 = S::ld_a(b1[u], k), y = Pair<S>::both_a(b0[u], b1[u], y0, y1, md, k);
 #pragma unroll
                 for (int g = 0; g < G; g++) {
                     const typename S::B x0 = S::ld_b(a0[g][u], k), x1 = S::ld_b(a1[g][u], k);
                     S::mac(acc[g][0], y0, x0, k);
-                    S::mac(acc[g][1], y1, x0, k);
-                    S::mac(acc[g][1], y0, x1, k);
+                    S::mac(acc[g][1], y, Pair<S>::both_b(a0[g][u], a1[g][u], x0, x1, md, k), k);
                     S::mac(acc[g][2], y1, x1, k);
                 }
             }
         }
     }
 #pragma unroll
-    for (int g = 0; g < G; g++)
+    for (int g = 0; g < G; g++) {
+        uint64_t r[3];
+#pragma unroll
+        for (int p = 0; p < 3; p++) r[p] = S::finish(acc[g][p], k);
+        r[1] = sub_mod(sub_mod(r[1], r[0], md.q), r[2], md.q);
 #pragma unroll
         for (int p = 0; p < 3; p++) {
-            const uint64_t r = S::finish(acc[g][p], k);
             uint64_t *out = a.out + (size_t)((g0 + g) * 3 + p) * a.l * N + o;
-            *out = a.first ? r : add_mod(r, *out, md.q);
+            *out = a.first ? r[p] : add_mod(r[p], *out, md.q);
         }
+    }
 }
-
-// FP64 products of primes below 2^41: 2048 of them stay below 2^53, so that no sum of a launch is brought back on the way
-struct SumFpLong : SumFp {
-    static constexpr int FLUSH = 2048;
-};
-static_assert(2 * SUM_TERMS <= SumFpLong::FLUSH);
 
 template <int G, int U, int MIN_CTAS>
 __global__ void __launch_bounds__(SUM_T, MIN_CTAS) multiply_sum_kernel(const __grid_constant__ SumArgs a) {
@@ -167,8 +208,8 @@ void launch_multiply_sum(const SumArgs &a, uint32_t queries, cudaStream_t s) {
     const dim3 grid((1u << a.logN) / SUM_T, a.l);
     switch (queries) {
         case 1: launch_k(multiply_sum_kernel<1, 4, 6>, grid, SUM_T, 0, s, a); break;
-        case 2: launch_k(multiply_sum_kernel<2, 3, 4>, grid, SUM_T, 0, s, a); break;
-        case 3: launch_k(multiply_sum_kernel<3, 3, 4>, grid, SUM_T, 0, s, a); break;
+        case 2: launch_k(multiply_sum_kernel<2, 5, 4>, grid, SUM_T, 0, s, a); break;
+        case 3: launch_k(multiply_sum_kernel<3, 4, 4>, grid, SUM_T, 0, s, a); break;
         default: launch_k(multiply_sum_kernel<4, 3, 4>, grid, SUM_T, 0, s, a); break;
     }
 }
