@@ -126,6 +126,8 @@ class rotary:
 
     def _apply(self, xs, plaintexts, galois_key, l):
         ctx, n, first = self.ctx, len(xs), xs[0]
+        # rotations read dense polynomials: of a view (the first limbs of a higher level) a dense copy is rotated and multiplied
+        xs = [x if x.data.is_contiguous() else x._like(x.data.contiguous().view(2, l, ctx.N)) for x in xs]
         terms = [[x] for x in xs] if self._vecs == 1 else [[x] + hoist_rotations(ctx, x, galois_key, [self.step, -self.step]) for x in xs]
         _, cts, held = _operands(ctx, terms)
         factors = [pt.data.contiguous() for i in range(n) for pt in (v[i] for v in plaintexts)]

@@ -1,0 +1,105 @@
+"""What rotary gives its kernels, and what it refuses, without a GPU: the native calls are replaced by ones that read the addresses
+that they are given the way the kernels do."""
+import ctypes
+import importlib
+import types
+
+import numpy as np
+import pytest
+import torch
+
+import pyPhantom as ph
+from pyPhantom import _native, rotary as rotary_class
+from pyPhantom import cache as cache_module
+
+rotary_module = importlib.import_module("pyPhantom.rotary")
+N, PRIME = 16, 1099511480321
+
+
+def _words(address, count):
+    return np.ctypeslib.as_array((ctypes.c_int64 * count).from_address(address)).copy()
+
+
+class _Native:
+    """the entries that rotated ciphertexts take; every ciphertext and plaintext that the products read is kept in `read`"""
+
+    def __init__(self):
+        self.read, self.calls = [], []
+
+    def b2_multiply_plain_sum(self, h, l, n, terms, cts, pts, out, stream):
+        self.calls.append("sum")
+        cts, pts = ((ctypes.c_uint64 * (n * terms)).from_address(a) for a in (cts, pts))
+        self.read.append([(_words(c, 2 * l * N), _words(p, l * N)) for c, p in zip(cts, pts)])
+        return 0
+
+    def b2_rescale_rounded_batch(self, *args):
+        return 0
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.calls.append(name)
+            return 0
+
+        return entry
+
+
+def _context(size_Q=4, bits=40):
+    ctx = types.SimpleNamespace(N=N, size_Q=size_Q, device=-1, _h=None, primes=np.full(size_Q + 1, PRIME, dtype=np.uint64),
+                                chain_bits=[bits * k for k in range(size_Q + 2)])
+    ctx.limbs_at = lambda k: size_Q - (k - 1)
+    ctx.empty = lambda *shape: torch.zeros((*shape, N), dtype=torch.int64)
+    return ctx
+
+
+@pytest.fixture
+def native(monkeypatch):
+    lib = _Native()
+    for module in (rotary_module, cache_module):
+        monkeypatch.setattr(module, "LIB", lib)
+        monkeypatch.setattr(module, "_stream", lambda: 0)
+    monkeypatch.setattr(_native, "_current_device", lambda: -1)
+
+    def hoist(ctx, ct, glk, steps):  # reads two dense polynomials behind the address, as the kernel does
+        x = torch.from_numpy(_words(ct.data.data_ptr(), 2 * ct._limbs * N)).reshape(2, ct._limbs, N)
+        return [ct._like(x + 1000 * s) for s in steps]
+
+    monkeypatch.setattr(rotary_module, "hoist_rotations", hoist)
+    return lib
+
+
+def _rotary(ctx, packing, scaling=1.0):
+    rot = object.__new__(rotary_class)  # without the tables, which lie on a device
+    rot.ctx, rot.packing, rot.scaling, rot._vecs, rot.step = ctx, packing, scaling, 1 if packing == "pairs" else 3, 1
+    return rot
+
+
+def _ciphertext(data, chain):
+    ct = ph.ciphertext()
+    ct._chain_index, ct._size, ct._limbs, ct._N, ct._scale, ct.data = chain, data.shape[0], data.shape[1], N, 2.0 ** 40, data
+    return ct
+
+
+def _plaintext(data, chain, scale=float(PRIME)):
+    pt = ph.plaintext()
+    pt._chain_index, pt._N, pt._limbs, pt._scale, pt.data = chain, N, data.shape[0], scale, data
+    return pt
+
+
+@pytest.mark.parametrize("packing", ["pairs", "halves", "interleaved"])
+@pytest.mark.parametrize("n", [1, 3, 17])
+def test_words_that_the_products_read(native, packing, n):
+    """ciphertexts whose polynomials lie apart (the first limbs of a higher level) count as what they hold, rotated or not"""
+    ctx, l = _context(), 3
+    rot = _rotary(ctx, packing)
+    high = torch.arange(n * 2 * 4 * N).reshape(n, 2, 4, N)
+    xs = [_ciphertext(x[:, :l] if i % 2 == 0 else x[:, :l].clone(), 2) for i, x in enumerate(high)]
+    pts = [[_plaintext(torch.full((l, N), 100 * v + i), 2) for i in range(n)] for v in range(rot._vecs)]
+    out = rot.apply(xs, pts, galois_key="key")
+    assert len(out) == n and all(ct.chain_index() == 3 and ct.scale() == 2.0 ** 40 for ct in out)
+    read = [pair for call in native.read for pair in call]
+    assert len(read) == n * rot._vecs
+    for i in range(n):
+        for v, offset in zip(range(rot._vecs), (0, 1000, -1000)):
+            ct, pt = read[i * rot._vecs + v]
+            assert np.array_equal(ct, high[i, :, :l].reshape(-1).numpy() + offset)
+            assert np.array_equal(pt, np.full(l * N, 100 * v + i))
