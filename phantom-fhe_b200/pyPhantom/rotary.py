@@ -114,7 +114,8 @@ class rotary:
             raise ValueError("Galois key not present")
         first, _, _ = _operands(ctx, [xs])
         l = first._limbs
-        if any(pt._chain_index != first._chain_index or pt.data.shape != (l, ctx.N) or pt.data.get_device() != ctx.device for v in plaintexts for pt in v):
+        if any(pt._chain_index != first._chain_index or pt.data.shape != (l, ctx.N) or pt.data.dtype != torch.int64 or pt.data.get_device() != ctx.device
+               for v in plaintexts for pt in v):
             raise ValueError("encrypted and plain parameter mismatch")
         if l < 2:
             raise ValueError("end of modulus switching chain reached")

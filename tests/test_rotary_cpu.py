@@ -103,3 +103,21 @@ def test_words_that_the_products_read(native, packing, n):
             ct, pt = read[i * rot._vecs + v]
             assert np.array_equal(ct, high[i, :, :l].reshape(-1).numpy() + offset)
             assert np.array_equal(pt, np.full(l * N, 100 * v + i))
+
+
+def _no_call(native, call, match):
+    with pytest.raises(ValueError, match=match):
+        call()
+    assert native.calls == [] and native.read == []
+
+
+@pytest.mark.parametrize("packing", ["pairs", "halves", "interleaved"])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.float64, torch.uint8])
+def test_plaintext_words_of_another_type(native, packing, dtype):
+    """words shorter than the kernel's would be read past their end"""
+    ctx, l = _context(), 3
+    rot = _rotary(ctx, packing)
+    xs = [_ciphertext(torch.zeros(2, l, N, dtype=torch.int64), 2) for _ in range(2)]
+    pts = [[_plaintext(torch.zeros(l, N, dtype=torch.int64), 2) for _ in range(2)] for _ in range(rot._vecs)]
+    pts[-1][1].data = torch.zeros(l, N, dtype=dtype)
+    _no_call(native, lambda: rot.apply(xs, pts, "key"), "mismatch")
