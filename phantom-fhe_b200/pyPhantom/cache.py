@@ -315,7 +315,7 @@ def cached_score_times_v(context, relin_key, galois_key, scores, cache, pages, m
         raise ValueError("ciphertext_cache: the cache belongs to another context")
     first, _, _ = _operands(ctx, [scores])
     _check_plain(first, mask_pt)
-    if mask_pt.data.shape != (first._limbs, ctx.N) or mask_pt.data.get_device() != ctx.device:
+    if mask_pt.data.shape != (first._limbs, ctx.N) or mask_pt.data.dtype != torch.int64 or mask_pt.data.get_device() != ctx.device:
         raise ValueError("encrypted and plain parameter mismatch")
     mask = mask_pt.data.contiguous()
     l, nominal, spread = first._limbs, first._scale, []

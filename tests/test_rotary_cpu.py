@@ -121,3 +121,13 @@ def test_plaintext_words_of_another_type(native, packing, dtype):
     pts = [[_plaintext(torch.zeros(l, N, dtype=torch.int64), 2) for _ in range(2)] for _ in range(rot._vecs)]
     pts[-1][1].data = torch.zeros(l, N, dtype=dtype)
     _no_call(native, lambda: rot.apply(xs, pts, "key"), "mismatch")
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.float64, torch.uint8])
+def test_mask_words_of_another_type(native, dtype):
+    ctx = _context()
+    cache = ph.ciphertext_cache(ctx, 1, 2)
+    cache._held, cache._free = [1, 1], []
+    score = _ciphertext(torch.zeros(2, 4, N, dtype=torch.int64), 1)
+    mask = _plaintext(torch.zeros(4, N, dtype=dtype), 1)
+    _no_call(native, lambda: ph.cached_score_times_v(ctx, None, None, [score], cache, [0], mask, 2, 4, 2), "mismatch")
