@@ -104,7 +104,8 @@ class rotary:
 
     def apply(self, xs, plaintexts, galois_key=None):
         """the ciphertexts xs (of one level and scale) rotated by the encoded factors, one level further down (rounded to nearest), at
-        their scale. "halves" and "interleaved" want Galois keys for the steps +-`step`."""
+        their scale: the plaintexts are at the prime's that the rescale removes, as `encode` makes them, and at no other. "halves" and
+        "interleaved" want Galois keys for the steps +-`step`."""
         ctx, vecs = self.ctx, self._vecs
         if len(plaintexts) != vecs or any(len(v) != len(xs) for v in plaintexts):
             raise ValueError("rotary: as many encoded factors as ciphertexts are wanted")
@@ -119,6 +120,9 @@ class rotary:
             raise ValueError("encrypted and plain parameter mismatch")
         if l < 2:
             raise ValueError("end of modulus switching chain reached")
+        prime = float(ctx.primes[l - 1])
+        if not all(abs(pt._scale - prime) <= 1e-9 * prime for v in plaintexts for pt in v):
+            raise ValueError("scale mismatch")
         out = []
         with on_device(ctx):
             for i in range(0, len(xs), CHUNK):

@@ -131,3 +131,15 @@ def test_mask_words_of_another_type(native, dtype):
     score = _ciphertext(torch.zeros(2, 4, N, dtype=torch.int64), 1)
     mask = _plaintext(torch.zeros(4, N, dtype=dtype), 1)
     _no_call(native, lambda: ph.cached_score_times_v(ctx, None, None, [score], cache, [0], mask, 2, 4, 2), "mismatch")
+
+
+@pytest.mark.parametrize("packing", ["pairs", "halves", "interleaved"])
+@pytest.mark.parametrize("scale", [2.0 ** 40, 2.0 ** 30, PRIME * 1.001, float("nan")])
+def test_plaintexts_at_another_scale(native, packing, scale):
+    """the rescale removes the prime: a result at the ciphertext's scale comes from plaintexts at the prime's"""
+    ctx, l = _context(), 3
+    rot = _rotary(ctx, packing)
+    xs = [_ciphertext(torch.zeros(2, l, N, dtype=torch.int64), 2) for _ in range(2)]
+    pts = [[_plaintext(torch.zeros(l, N, dtype=torch.int64), 2) for _ in range(2)] for _ in range(rot._vecs)]
+    pts[-1][0].set_scale(scale)
+    _no_call(native, lambda: rot.apply(xs, pts, "key"), "scale mismatch")
