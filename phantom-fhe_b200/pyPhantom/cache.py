@@ -243,6 +243,14 @@ class ciphertext_cache:
 BATCH = 16  # ciphertexts that go through each kernel together (the products of one call of b2_multiply_relin_rescale_many)
 
 
+def _nominal(scale, prime):
+    """A product keeps its first factor's (nominal) scale, as the lists' forms label it, which is right where the other factor's
+    scale is about the prime that the rescale removes. The primes of a size lie within a few per cent of the power of two that such
+    a scale is (24 primes of 30 bits for N = 2^17: 6); an eighth away is another size."""
+    if not 0.875 < scale / float(prime) < 1.125:
+        raise ValueError("scale mismatch")
+
+
 def _rotate_add_batch(ctx, x, step, galois_key):
     """x[n][2][l][N] += x rotated by `step`, every kernel one launch over the n ciphertexts"""
     n, l = x.shape[0], x.shape[2]
@@ -262,7 +270,7 @@ def cached_qkt(context, relin_key, galois_key, q, cache, pages, d_head, plane=0)
     """compute_qkt (src/attention.cu:10-28) over cached pages: per page q * k, one rescale, the sum over each d_head block; slot
     t * d_total + h * d_head of result j holds Q[h] . K of position t of page pages[j]. The pages are read where they lie, at q's
     level or above it, and every kernel runs over 16 of them at a time; the rescale rounds to nearest, so that the results agree
-    with compute_qkt's to rounding, not limb for limb."""
+    with compute_qkt's to rounding, not limb for limb. They keep q's scale: the pages' has to be about the prime that it removes."""
     ctx, pages = context, cache._live(pages)
     plane = cache._plane(plane)
     if d_head == 0 or d_head & (d_head - 1):
@@ -275,6 +283,7 @@ def cached_qkt(context, relin_key, galois_key, q, cache, pages, d_head, plane=0)
     if q._chain_index == ctx.size_Q:
         raise ValueError("end of modulus switching chain reached")
     l, nominal, results = q._limbs, q._scale, []
+    _nominal(cache._scale, ctx.primes[l - 1])
     tab = _key_table(ctx, relin_key, l)
     step = cache._page_bytes
     base = cache.data.data_ptr() + plane * cache.pages() * step
@@ -301,7 +310,8 @@ def cached_score_times_v(context, relin_key, galois_key, scores, cache, pages, m
     """score_times_v (src/attention.cu:30-98) over cached pages: sum_t score[t] V[t]. The masked scores are spread over their heads
     16 at a time; the products with all pages are summed before they are relinearised, so that one relinearisation, one rescale
     and one fold over the positions serve the whole context (score_times_v makes each of them per chunk). Same levels; the
-    rescales round to nearest."""
+    rescales round to nearest. The result keeps the scores' scale: the mask's and the pages' have to be about the primes that are
+    removed."""
     ctx = context
     if len(scores) == 0:
         raise ValueError("score_times_v: score_cts is empty")
@@ -319,8 +329,11 @@ def cached_score_times_v(context, relin_key, galois_key, scores, cache, pages, m
         raise ValueError("encrypted and plain parameter mismatch")
     mask = mask_pt.data.contiguous()
     l, nominal, spread = first._limbs, first._scale, []
-    if l < 3:
+    deep = min(l - 1, cache._limbs)  # of the products
+    if l < 3 or deep < 2:
         raise ValueError("end of modulus switching chain reached")
+    _nominal(mask_pt._scale, ctx.primes[l - 1])
+    _nominal(cache._scale, ctx.primes[deep - 1])
     with on_device(ctx):
         for p0 in range(0, len(scores), BATCH):
             x = torch.stack([s.data for s in scores[p0:p0 + BATCH]])

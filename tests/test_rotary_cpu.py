@@ -143,3 +143,36 @@ def test_plaintexts_at_another_scale(native, packing, scale):
     pts = [[_plaintext(torch.zeros(l, N, dtype=torch.int64), 2) for _ in range(2)] for _ in range(rot._vecs)]
     pts[-1][0].set_scale(scale)
     _no_call(native, lambda: rot.apply(xs, pts, "key"), "scale mismatch")
+
+
+def _pages(ctx, scale, chain=1):
+    cache = ph.ciphertext_cache(ctx, chain, 2, scale=scale)
+    cache._held, cache._free = [1, 1], []
+    return cache
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 38, 2.0 ** 39, 2.0 ** 41, 2.0 ** 50])
+def test_pages_and_masks_at_a_scale_that_the_rescale_does_not_remove(native, scale):
+    """the products over pages keep the nominal scale, which holds where the other factor's scale is about the removed prime"""
+    ctx = _context()
+    ct = _ciphertext(torch.zeros(2, 4, N, dtype=torch.int64), 1)
+    mask = lambda s: _plaintext(torch.zeros(4, N, dtype=torch.int64), 1, s)
+    _no_call(native, lambda: ph.cached_qkt(ctx, None, None, ct, _pages(ctx, scale), [0], 2), "scale mismatch")
+    _no_call(native, lambda: ph.cached_score_times_v(ctx, None, None, [ct], _pages(ctx, scale), [0], mask(float(PRIME)), 2, 4, 2), "scale mismatch")
+    _no_call(native, lambda: ph.cached_score_times_v(ctx, None, None, [ct], _pages(ctx, 2.0 ** 40), [0], mask(scale), 2, 4, 2), "scale mismatch")
+
+
+def test_the_prime_that_each_product_over_pages_removes(native):
+    """primes of several sizes: the score's, the mask's and the pages' scales go with the primes of their own levels"""
+    ctx = _context()
+    ctx.primes = np.array([1 << 60, 1 << 50, 1 << 45, 1 << 40, 1 << 30], dtype=np.uint64)
+    ct = _ciphertext(torch.zeros(2, 4, N, dtype=torch.int64), 1)
+    mask = _plaintext(torch.zeros(4, N, dtype=torch.int64), 1, 2.0 ** 40)
+    for chain, scale in ((1, 2.0 ** 45), (3, 2.0 ** 50)):  # pages at the masked scores' level or above, or one below
+        for wrong in (2.0 ** 40, 2.0 ** 60):
+            _no_call(native, lambda: ph.cached_score_times_v(ctx, None, None, [ct], _pages(ctx, wrong, chain), [0], mask, 2, 4, 2), "scale mismatch")
+        with pytest.raises(AttributeError):  # past the checks: no key was given
+            ph.cached_score_times_v(ctx, None, None, [ct], _pages(ctx, scale, chain), [0], mask, 2, 4, 2)
+        native.calls.clear()
+    with pytest.raises(AttributeError):
+        ph.cached_qkt(ctx, None, None, ct, _pages(ctx, 2.0 ** 40), [0], 2)
