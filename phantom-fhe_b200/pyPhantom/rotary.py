@@ -13,6 +13,7 @@ t * heads * d_head + h * d_head + i of a ciphertext holds element i of head h at
 Elements of a head beyond its pairs pass unchanged. Positions that are dropped (`keep`), and slots of no position, come out as zeros:
 a decoding step's one position goes into its place of a page that way, without a mask of its own.
 """
+import math
 from array import array
 
 import torch
@@ -72,7 +73,13 @@ class rotary:
 
     def encode(self, encoder, factors, chain_index):
         """[vector][ciphertext] plaintexts of `factors` at a level, at the scale of the prime that the rescale after the product
-        removes. Queries and keys of all layers at that level and of these positions share them."""
+        removes. Queries and keys of all layers at that level and of these positions share them. Values too large for a plaintext,
+        and what is no finite number, are refused; for that the host waits for the factors. While a graph is captured it cannot, and
+        takes them as they are."""
+        return self._encode(encoder, factors, chain_index, False)
+
+    def _encode(self, encoder, factors, chain_index, made_here):
+        """made_here: the values are this object's, of finite positions"""
         ctx = self.ctx
         if factors.dim() != 3 or factors.dtype != torch.complex128 or factors.shape[2] != ctx.N // 2:
             raise ValueError("rotary: factors are complex128 [vectors][ciphertexts][slots]")
@@ -87,11 +94,18 @@ class rotary:
         if scale * max(1.0, abs(self.scaling)) * 1.4143 >= 2.0 ** 61:  # no coefficient exceeds it, and none may pass 62 bits
             raise ValueError("scale out of bounds")
         vecs, n = factors.shape[0], factors.shape[1]
-        if n == 0:
+        if vecs == 0 or n == 0:
             return [[] for _ in range(vecs)]
         vals = factors.to(device=ctx.device).clone(memory_format=torch.contiguous_format)  # overwritten by the transform
         coeffs, data = torch.empty(vecs * n, ctx.N, dtype=torch.int64, device=ctx.device), ctx.empty(vecs, n, l)
         with on_device(ctx):
+            largest = max(1.0, abs(self.scaling))
+            if not made_here and not torch.cuda.is_current_stream_capturing():
+                low, high = torch.view_as_real(vals).aminmax()
+                largest = float(torch.maximum(-low, high))  # NaN if there is one
+            bound = 1.4143 * largest * scale
+            if not (bound < 2.0 ** 61 and math.log2(max(bound, 1.0)) + 2 < ctx.chain_bits[l]):
+                raise ValueError("encoded values are too large")
             check(LIB.b2_encode_coeffs_batch(ctx._h, vecs * n, vals.data_ptr(), encoder._d_rot.data_ptr(), encoder._d_ksi.data_ptr(), scale / encoder.slots,
                                              coeffs.data_ptr(), _stream()))
             check(LIB.b2_expand_single_chain_batch(ctx._h, l, vecs * n, coeffs.data_ptr(), data.data_ptr(), _stream()))
@@ -152,5 +166,5 @@ class rotary:
             part = xs[i:i + CHUNK]
             if any(x._chain_index != part[0]._chain_index for x in part):
                 raise ValueError("encrypted and plain parameter mismatch")
-            out += self.apply(part, self.encode(encoder, f[:, i:i + CHUNK], part[0]._chain_index), galois_key)
+            out += self.apply(part, self._encode(encoder, f[:, i:i + CHUNK], part[0]._chain_index, True), galois_key)
         return out

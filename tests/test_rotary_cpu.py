@@ -2,6 +2,7 @@
 that they are given the way the kernels do."""
 import ctypes
 import importlib
+import math
 import types
 
 import numpy as np
@@ -176,3 +177,39 @@ def test_the_prime_that_each_product_over_pages_removes(native):
         native.calls.clear()
     with pytest.raises(AttributeError):
         ph.cached_qkt(ctx, None, None, ct, _pages(ctx, 2.0 ** 40), [0], 2)
+
+
+def _encoder(ctx):
+    ctx.device = "cpu"  # tensors are made on it
+    return types.SimpleNamespace(ctx=ctx, slots=ctx.N // 2, _d_rot=torch.zeros(1), _d_ksi=torch.zeros(1))
+
+
+@pytest.mark.parametrize("value,at", [(1e9, (0, 0, 0)), (-1e9j, (2, 1, 7)), (math.inf, (0, 1, 3)), (complex(0, -math.inf), (1, 0, 0)), (math.nan, (0, 0, 7)),
+                                      (complex(1, math.nan), (2, 0, 2))])
+def test_factors_that_no_plaintext_holds(native, monkeypatch, value, at):
+    """coefficients past 62 bits, and what is no number, are refused as the encoder refuses them: a coefficient is at most the scale
+    times the largest part times sqrt(2)"""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(_native, "_current_device", lambda: "cpu")
+    ctx = _context()
+    rot, factors = _rotary(ctx, "halves"), torch.ones(3, 2, N // 2, dtype=torch.complex128)
+    assert [len(v) for v in rot.encode(_encoder(ctx), factors, 2)] == [2, 2, 2]
+    native.calls.clear()
+    factors[at] = value
+    _no_call(native, lambda: rot.encode(_encoder(ctx), factors, 2), "encoded values are too large")
+
+
+def test_factors_as_large_as_a_plaintext_holds(native, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(_native, "_current_device", lambda: "cpu")
+    ctx = _context(bits=42)  # two limbs hold 84 bits: the 62 of a coefficient come first
+    rot, factors = _rotary(ctx, "pairs"), torch.zeros(1, 1, N // 2, dtype=torch.complex128)
+    most = 2.0 ** 61 / (1.4143 * PRIME)
+    factors[0, 0, 3] = complex(0.5, -0.999 * most)
+    rot.encode(_encoder(ctx), factors, 3)
+    factors[0, 0, 3] = complex(0.5, -1.001 * most)
+    native.calls.clear()
+    _no_call(native, lambda: rot.encode(_encoder(ctx), factors, 3), "encoded values are too large")
+    ctx = _context(bits=21)  # two limbs hold 42 bits
+    factors[0, 0, 3] = 1.0
+    _no_call(native, lambda: _rotary(ctx, "pairs").encode(_encoder(ctx), factors, 3), "encoded values are too large")
