@@ -38,6 +38,8 @@ class rotary:
             raise ValueError("rotary: heads * d_head must be in [1, slots]")
         if pairs < 1 or pairs > (d_head if packing == "pairs" else d_head // 2):
             raise ValueError("rotary: more pairs than a head holds")
+        if not (math.isfinite(scaling) and bool(torch.isfinite(f * 2.0 ** 64).all())):  # the angle of any integer position
+            raise ValueError("rotary: the angles per position and the scaling must be finite (below 2^960)")
         a = [0] * pairs if axes is None else [int(v) for v in axes]
         if len(a) != pairs or min(a) < 0:
             raise ValueError("rotary: an axis for every pair is wanted")

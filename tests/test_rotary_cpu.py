@@ -213,3 +213,15 @@ def test_factors_as_large_as_a_plaintext_holds(native, monkeypatch):
     ctx = _context(bits=21)  # two limbs hold 42 bits
     factors[0, 0, 3] = 1.0
     _no_call(native, lambda: _rotary(ctx, "pairs").encode(_encoder(ctx), factors, 3), "encoded values are too large")
+
+
+@pytest.mark.parametrize("bad", [dict(inv_freq=[1.0, math.nan]), dict(inv_freq=[math.inf, 1.0]), dict(inv_freq=[1.0, -1e300]), dict(scaling=math.nan),
+                                 dict(scaling=math.inf)])
+def test_angles_that_are_no_numbers(monkeypatch, bad):
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device: None)
+    good = dict(inv_freq=[1.0, -0.5], heads=2, d_head=4, packing="pairs")
+    ctx = types.SimpleNamespace(N=N, device="cpu")
+    rotary_class(ctx, **good)
+    rotary_class(ctx, **{**good, "scaling": -2.0, "inv_freq": [1e280, 0.0]})
+    with pytest.raises(ValueError, match="finite"):
+        rotary_class(ctx, **{**good, **bad})
