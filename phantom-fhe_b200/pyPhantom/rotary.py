@@ -47,6 +47,10 @@ class rotary:
         self.n_axes = max(a) + 1
         self.positions_per_ct = context.N // 2 // (heads * d_head)
         self.inv_freq, self.axes = f, torch.tensor(a, dtype=torch.int32, device=context.device)
+        steepest = {}  # the largest angle per position on each axis that a pair follows
+        for axis, angle in zip(a, f.abs().tolist()):
+            steepest[axis] = max(steepest.get(axis, 0.0), angle)
+        self._followed, self._steepest = torch.tensor(list(steepest), device=f.device), torch.tensor(list(steepest.values()), dtype=torch.float64, device=f.device)
         self.step = pairs if packing == "halves" else 1
         self._vecs = 1 if packing == "pairs" else 3
         torch.cuda.synchronize(context.device)  # the tables are there for whichever stream comes first
@@ -159,10 +163,13 @@ class rotary:
         return [first._like(z, chain_index=first._chain_index + 1, scale=x._scale) for x, z in zip(xs, out.unbind(0))]
 
     def forward(self, encoder, xs, positions, keep=None, conjugate=False, galois_key=None):
-        """factors, encode and apply for ciphertexts of one level, CHUNK of them at a time"""
+        """factors, encode and apply for ciphertexts of one level, CHUNK of them at a time. A kept position that is not finite would
+        spoil its whole ciphertext and is refused; for that the host waits for positions in floating point, except while a graph is
+        captured."""
         f = self.factors(positions, keep, conjugate)
         if f.shape[1] != len(xs):
             raise ValueError("rotary: positions for ceil(tokens / positions_per_ct) ciphertexts were given")
+        self._check_finite(positions, keep)
         out = []
         for i in range(0, len(xs), CHUNK):
             part = xs[i:i + CHUNK]
@@ -170,3 +177,14 @@ class rotary:
                 raise ValueError("encrypted and plain parameter mismatch")
             out += self.apply(part, self._encode(encoder, f[:, i:i + CHUNK], part[0]._chain_index, True), galois_key)
         return out
+
+    def _check_finite(self, positions, keep):
+        if not positions.dtype.is_floating_point:  # every integer's angle is
+            return
+        with on_device(self.ctx):
+            if torch.cuda.is_current_stream_capturing():
+                return
+            p = (positions if positions.dim() == 2 else positions[:, None])[:, self._followed].double()
+            bad = ~torch.isfinite(p * self._steepest).all(1)
+            if bool((bad if keep is None else bad & keep).any()):
+                raise ValueError("rotary: a kept position is not finite")

@@ -225,3 +225,56 @@ def test_angles_that_are_no_numbers(monkeypatch, bad):
     rotary_class(ctx, **{**good, "scaling": -2.0, "inv_freq": [1e280, 0.0]})
     with pytest.raises(ValueError, match="finite"):
         rotary_class(ctx, **{**good, **bad})
+
+
+class _Rotary(rotary_class):
+    """on the host: factors of nothing, and what forward would do with them is counted"""
+
+    def factors(self, positions, keep=None, conjugate=False):
+        return torch.ones(1, 1, N // 2, dtype=torch.complex128)
+
+    def _encode(self, *args):
+        return [["plaintext"]]
+
+    def apply(self, xs, plaintexts, galois_key=None):
+        return list(xs)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_kept_positions_that_are_no_numbers(monkeypatch, dtype, bad):
+    """they would spoil every slot of their ciphertext; in a dropped position's place, or on an axis that no pair follows, they do not count"""
+    capturing = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(capturing))
+    monkeypatch.setattr(_native, "_current_device", lambda: "cpu")
+    rot = _Rotary(types.SimpleNamespace(N=N, device="cpu"), [1.0, 0.5], 2, 4, axes=[0, 2])
+    x = types.SimpleNamespace(_chain_index=1)
+    p = torch.ones(3, 3, dtype=dtype)
+    assert rot.forward(None, [x], p) == [x]
+    p[:, 1] = bad
+    assert rot.forward(None, [x], p) == [x]
+    keep = torch.tensor([True, False, True])
+    p[1, 2] = bad
+    assert rot.forward(None, [x], p, keep=keep) == [x]
+    for k in (None, ~keep):
+        with pytest.raises(ValueError, match="finite"):
+            rot.forward(None, [x], p, keep=k)
+    capturing.append(1)  # the host cannot look
+    assert rot.forward(None, [x], p) == [x]
+    one = _Rotary(types.SimpleNamespace(N=N, device="cpu"), [0.0, 2.0], 2, 4)
+    capturing.clear()
+    with pytest.raises(ValueError, match="finite"):
+        one.forward(None, [x], p[:, 2])
+    assert one.forward(None, [x], p[:1, 2]) == [x] and one.forward(None, [x], p[:, 2].nan_to_num(0, 0, 0).long()) == [x]
+
+
+def test_angles_past_the_doubles(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(_native, "_current_device", lambda: "cpu")
+    rot = _Rotary(types.SimpleNamespace(N=N, device="cpu"), [1e-200, -1e250, 1e-3], 2, 4, axes=[0, 0, 1])
+    x = types.SimpleNamespace(_chain_index=1)
+    assert rot.forward(None, [x], torch.tensor([[1e50, 1e300]], dtype=torch.float64)) == [x]
+    with pytest.raises(ValueError, match="finite"):
+        rot.forward(None, [x], torch.tensor([[1e60, 0.0]], dtype=torch.float64))
