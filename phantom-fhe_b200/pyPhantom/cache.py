@@ -199,6 +199,8 @@ class ciphertext_cache:
             with on_device(self.ctx):
                 check(LIB.b2_pages_move(self.ctx._h, self._limbs, self._planes, data.data_ptr(), pages, self.data.data_ptr(), self._limbs, len(self._held),
                                         len(live), at, at, _stream()))
+        # the pool may have been made on another stream: its memory goes back only after what this one still does with it
+        self.data.record_stream(torch.cuda.current_stream(self.ctx.device))
         self.data = data
         self._held = self._held[:n] + [0] * (pages - n)
         self._free = [p for p, k in enumerate(self._held) if not k]
