@@ -187,10 +187,14 @@ class ciphertext_cache:
         return [[new[p] for p in t] for t in tables]
 
     def resize(self, pages):
-        """another number of pages; those allocated have to lie in front of it (`compact`)"""
+        """another number of pages; those allocated have to lie in front of it (`compact`). The pool moves: a graph captured before
+        works on memory that was given back, and has to be captured anew; while one is captured this call is refused."""
         pages = int(pages)
         if pages < 1 or any(self._held[pages:]):
             raise ValueError("ciphertext_cache: allocated pages lie behind the new end (compact first)")
+        with on_device(self.ctx):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("ciphertext_cache: resize cannot be captured (every replay would read the memory that it gives back)")
         n = min(pages, len(self._held))
         data = self.ctx.empty(self._planes, pages, 2, self._limbs)
         live = array("q", [p for p in range(n) if self._held[p]])

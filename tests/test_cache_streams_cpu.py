@@ -1,4 +1,4 @@
-"""What a cache does to the memory that it gives back, without a GPU: on which stream."""
+"""What a cache does to the memory that it gives back, without a GPU: on which stream, and not while a graph is captured."""
 import types
 
 import pytest
@@ -42,3 +42,12 @@ def test_resize_holds_the_old_memory_until_it_is_read(cache):
     cache.resize(4)
     assert len(cache.calls) == 1 and cache.pages() == 4 and cache.data is not old
     assert old.streams == ["the stream that resize works on"]
+
+
+def test_resize_is_not_captured(cache, monkeypatch):
+    """a graph would read the memory given back here at every replay"""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    old = cache.data
+    with pytest.raises(RuntimeError, match="captured"):
+        cache.resize(4)
+    assert cache.data is old and cache.pages() == 6 and cache.free_pages() == 3 and cache.calls == []
