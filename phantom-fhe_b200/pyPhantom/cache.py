@@ -11,6 +11,7 @@ stream at a time; calls work on torch's current stream of the context's device. 
 replays the moves of the numbers it was captured with.
 """
 import heapq
+import math
 from array import array
 from operator import index
 
@@ -28,6 +29,8 @@ class ciphertext_cache:
             raise ValueError("ciphertext_cache: at least one page and one plane are wanted")
         if not 1 <= chain_index <= context.size_Q:
             raise ValueError("chain index out of range")
+        if not 0 < float(scale) < math.inf:
+            raise ValueError("scale out of bounds")
         self.ctx, self._chain_index, self._limbs, self._scale = context, int(chain_index), context.limbs_at(chain_index), float(scale)
         self._planes, self._page_bytes = planes, 16 * self._limbs * context.N
         self.data = context.empty(planes, pages, 2, self._limbs)
@@ -165,7 +168,7 @@ class ciphertext_cache:
         other = self if source is None else source
         if other.ctx is not self.ctx or other._planes != self._planes or other._limbs < self._limbs:
             raise ValueError("ciphertext_cache: the source has another context, other planes or a lower level")
-        if abs(other._scale - self._scale) > 1e-9 * self._scale:
+        if not abs(other._scale - self._scale) <= 1e-9 * self._scale:
             raise ValueError("scale mismatch")
         dst = self._live(dst)
         if any(self._held[p] > 1 for p in dst):
@@ -220,7 +223,7 @@ class ciphertext_cache:
             raise ValueError("ciphertext_cache: a two-polynomial ciphertext in NTT form on the context's device is wanted")
         if ct._chain_index > self._chain_index or ct._limbs < self._limbs:
             raise ValueError("cannot switch to higher level modulus")
-        if abs(ct._scale - self._scale) > 1e-9 * self._scale:
+        if not abs(ct._scale - self._scale) <= 1e-9 * self._scale:
             raise ValueError("scale mismatch")
         return page
 

@@ -1,4 +1,5 @@
-"""What a cache does to the memory that it gives back, without a GPU: on which stream, and not while a graph is captured."""
+"""What a cache does to the memory that it gives back, without a GPU: on which stream, and not while a graph is captured. And which
+scales it takes."""
 import types
 
 import pytest
@@ -51,3 +52,20 @@ def test_resize_is_not_captured(cache, monkeypatch):
     with pytest.raises(RuntimeError, match="captured"):
         cache.resize(4)
     assert cache.data is old and cache.pages() == 6 and cache.free_pages() == 3 and cache.calls == []
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 0.0, -2.0 ** 40])
+def test_scales_that_are_no_scales(cache, scale):
+    """NaN compares as unequal to nothing: neither a cache nor what goes into one may have it"""
+    with pytest.raises(ValueError, match="scale out of bounds"):
+        ph.ciphertext_cache(cache.ctx, 1, 2, scale=scale)
+    ct = cache.page(1).clone()
+    ct.set_scale(scale)
+    other = ph.ciphertext_cache(cache.ctx, 1, 6, 2)
+    other.allocate(6)
+    other._scale = scale
+    cache.calls.clear()
+    for call in (lambda: cache.store(0, ct), lambda: cache.append(0, ct), lambda: cache.copy([0], [0], source=other)):
+        with pytest.raises(ValueError, match="scale mismatch"):
+            call()
+    assert cache.calls == [] and not bool(cache.data.any())
