@@ -2726,6 +2726,9 @@ extern "C" int b2_multiply_plain_sum(b2_ctx *c, size_t l, size_t n, size_t terms
     bool ok = aligned32(d_out);
     for (size_t i = 0; i < n * terms; i++) ok = ok && d_ct[i] && d_pt[i] && aligned32(d_ct[i]) && aligned32(d_pt[i]);
     if (!ok) return fail(B2_EINVAL, "multiply_plain_sum: operands must be there and 32-byte aligned");
+    const auto overlaps = [&](const uint64_t *x, size_t polys) { return x < d_out + n * 2 * l * c->N && d_out < x + polys * l * c->N; };
+    for (size_t i = 0; i < n * terms; i++) ok = ok && !overlaps(d_ct[i], 2) && !overlaps(d_pt[i], 1);
+    if (!ok) return fail(B2_EINVAL, "multiply_plain_sum: the result overlaps an operand");
     for (size_t i = 0; i < n; i += PLAIN_SETS) {
         const size_t m = std::min<size_t>(PLAIN_SETS, n - i);
         PlainSumArgs a{};

@@ -6,6 +6,8 @@ import torch
 pytestmark = pytest.mark.gpu
 
 import pyPhantom as ph
+from pyPhantom._native import LIB, check
+from gpu_helpers import stream
 
 
 @pytest.fixture(scope="module")
@@ -39,3 +41,25 @@ def test_rotated_views(kit, packing):
     want = rot.forward(enc, dense, pos, galois_key=kit["glk"])
     for g, w in zip(got, want):
         assert torch.equal(g.data, w.data) and bool(g.data.any())
+
+
+def test_plain_sums_onto_their_operands(kit):
+    """the result of a batch may not lie on what a later launch of it still reads"""
+    ctx, l = kit["ctx"], 2
+    one = 8 * ctx.N
+    pool = torch.zeros(8, l, ctx.N, dtype=torch.int64, device="cuda")
+    at = pool.data_ptr()
+
+    def call(out, cts, pts):
+        a, b = (np.array(v, dtype=np.uint64) for v in (cts, pts))
+        check(LIB.b2_multiply_plain_sum(ctx._h, l, len(a), 1, a.ctypes.data, b.ctypes.data, out, stream()))
+
+    poly = lambda k: at + k * l * one  # a ciphertext takes two, a plaintext one, the two results four
+    for out, cts, pts in [(0, [4, 3], [6, 7]), (2, [0, 1], [6, 7]), (0, [4, 4], [6, 3]), (4, [0, 2], [4, 3]), (0, [2, 4], [6, 7])]:
+        with pytest.raises(ValueError, match="overlaps"):
+            call(poly(out), [poly(k) for k in cts], [poly(k) for k in pts])
+    with pytest.raises(ValueError, match="overlaps"):  # by a little
+        call(poly(0), [poly(4), poly(4) - 32], [poly(6), poly(7)])
+    call(poly(0), [poly(4)] * 2, [poly(6), poly(7)])
+    call(poly(4), [poly(2)] * 2, [poly(0), poly(3)])
+    assert not bool(pool.any())
