@@ -70,6 +70,8 @@ class rotary:
             raise ValueError("rotary: keep is one truth value a token")
         if p.get_device() != ctx.device or (keep is not None and keep.get_device() != ctx.device):
             raise ValueError("rotary: positions and keep must lie on the context's device")
+        if p.is_neg():  # the imaginary part of a conjugate: its words are not its values
+            p = p.resolve_neg()
         out = torch.empty(self._vecs, -(-tokens // self.positions_per_ct), ctx.N // 2, dtype=torch.complex128, device=ctx.device)
         with on_device(ctx):
             check(LIB.b2_rotary_factors(ctx._h, _PACKINGS[self.packing], tokens, self.heads, self.d_head, self.pairs, p.data_ptr(), kind, p.stride(0),

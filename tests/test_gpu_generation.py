@@ -63,3 +63,12 @@ def test_plain_sums_onto_their_operands(kit):
     call(poly(0), [poly(4)] * 2, [poly(6), poly(7)])
     call(poly(4), [poly(2)] * 2, [poly(0), poly(3)])
     assert not bool(pool.any())
+
+
+def test_positions_that_torch_negates_on_the_fly(kit):
+    """the imaginary part of a conjugate is a view with a bit instead of a sign"""
+    rot = ph.rotary(kit["ctx"], [1.0, 0.1], 8, 16)
+    z = torch.complex(torch.zeros(5, dtype=torch.float64, device="cuda"), torch.arange(5, dtype=torch.float64, device="cuda"))
+    p = z.conj().imag
+    assert p.is_neg()
+    assert torch.equal(rot.factors(p), rot.factors(p.clone())) and not torch.equal(rot.factors(p), rot.factors(z.imag))
