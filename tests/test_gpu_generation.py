@@ -8,6 +8,7 @@ pytestmark = pytest.mark.gpu
 import pyPhantom as ph
 from pyPhantom._native import LIB, check
 from gpu_helpers import stream
+from test_gpu_cache import MIXED, _below, _ct, _ctx, _residues
 
 
 @pytest.fixture(scope="module")
@@ -72,3 +73,49 @@ def test_positions_that_torch_negates_on_the_fly(kit):
     p = z.conj().imag
     assert p.is_neg()
     assert torch.equal(rot.factors(p), rot.factors(p.clone())) and not torch.equal(rot.factors(p), rot.factors(z.imag))
+
+
+# ---- several queries in every arithmetic ------------------------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def pool():
+    """three scores and three pages of the eight primes of every arithmetic (61 to 30 bits), the first of each the largest residues
+    throughout, and the nine products of a score and a page in integers of any size"""
+    ctx = _ctx(MIXED + _below(60, 2)[1:])
+    rng = np.random.default_rng(21)
+    q = np.array(MIXED, dtype=object)[:, None]
+    sides = []
+    for _ in range(2):
+        x = _residues(rng, ctx, 3, 2, 8)
+        x[0] = ctx.primes[:8].astype(np.uint64)[:, None] - np.uint64(1)
+        sides.append(x)
+    a, b = (x.astype(object) for x in sides)
+    products = [[[u[0] * v[0] % q, (u[0] * v[1] + u[1] * v[0]) % q, u[1] * v[1] % q] for v in b] for u in a]
+    return ctx, q, [_ct(ctx, x) for x in sides[0]], sides[1], products
+
+
+@pytest.mark.parametrize("queries", [1, 2, 3, 4, 5, 7])
+@pytest.mark.parametrize("terms", [1, 7, 8, 9, 15, 30, 60, 61, 64, 65, 129])
+def test_long_sums_of_several_queries(pool, queries, terms):
+    """past what the sums in registers take before they are brought back (7 products below 2^50, 60 below 2^41, 8 and 31 above) and
+    into a second and third launch, which add to the first one's results. The first query's operands are the largest residues in
+    every term, the others' are drawn for every term of every query: an operand read in another's place shows"""
+    ctx, q, scores, pages, products = pool
+    rng = np.random.default_rng(100 * queries + terms)
+    cache = ph.ciphertext_cache(ctx, 1, 5)
+    cache.allocate(5)
+    held = [0, 1, 2, 0, 1]
+    for p, k in enumerate(held):
+        cache.data[0, p].copy_(torch.from_numpy(pages[k].view(np.int64)))
+    for largest in (True, False):
+        pick = rng.integers(0, 3, (queries, terms))
+        table = [0] * terms if largest else [int(p) for p in rng.integers(0, 5, terms)]
+        if largest:
+            pick[0] = 0
+        got = cache.multiply_sum([[scores[k] for k in row] for row in pick], table)
+        assert len(got) == queries
+        for g in range(queries):
+            count = np.zeros((3, 3), dtype=int)
+            np.add.at(count, (pick[g], [held[p] for p in table]), 1)
+            for p in range(3):
+                want = sum(int(count[i, j]) * products[i][j][p] for i in range(3) for j in range(3) if count[i, j]) % q
+                assert np.array_equal(got[g].numpy()[p], want.astype(np.uint64)), (largest, g, p)
