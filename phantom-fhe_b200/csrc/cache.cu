@@ -10,7 +10,7 @@ namespace b2 {
 // ---- pages ------------------------------------------------------------------------------------------------------------
 // A thread owns the same 32 bytes of every page and walks its lane's steps, so that moves of a pool onto itself need no second
 // buffer and no order between threads. Loads of a batch of steps go out before its stores: no step reads what an earlier step of
-// the plan wrote, whichever is issued first. Steps of one source that follow one another read it once.
+// the plan wrote, whichever is issued first. Steps of one source that follow one another in a batch read it once.
 // Bound by HBM: a copy's rate, half reads and half writes. Four steps a batch take 56 registers, so that an SM has 1024 threads with
 // 128 bytes each in flight: 47 pages of 2 MB in four planes change places in 121 us (6.5 TB/s); with eight steps (126 registers, 512
 // threads) in 159, with two in 130.
@@ -19,7 +19,6 @@ struct PageMoves {  // 4 KB of parameters: they cost a launch less than 0.1 us o
     uint16_t end[PAGE_LANES];
     PageStep step[PAGE_STEPS];
 };
-constexpr int PAGE_BATCH = 4;
 
 __global__ void __launch_bounds__(256, 4) pages_move_kernel(const __grid_constant__ PageMoves m) {
     pdl_enter();

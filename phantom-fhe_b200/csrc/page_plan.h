@@ -10,6 +10,7 @@ namespace b2 {
 
 // A step stores the words of page `src` to page `dst`. Two names stand for no page: PAGE_ZERO as a source is a page of zeros,
 // PAGE_KEPT is a value that a thread holds on to: as a destination it takes the source's word, as a source it gives it back.
+constexpr int PAGE_BATCH = 4;  // steps whose loads go out before their stores
 constexpr uint32_t PAGE_ZERO = 0xFFFFFFFFu, PAGE_KEPT = 0xFFFFFFFEu, PAGE_MAX = 0xFFFFFFF0u;
 struct PageStep {
     uint32_t src, dst;
@@ -42,7 +43,7 @@ inline PagePlan plan_pages(size_t n, const int64_t *dst, const int64_t *src, boo
         std::sort(pages.begin(), pages.end());
         free_of_order = std::none_of(op.begin(), op.end(), [&](uint32_t i) { return src[i] >= 0 && std::binary_search(pages.begin(), pages.end(), src[i]); });
     }
-    if (free_of_order) {  // steps of one source side by side: it is read once
+    if (free_of_order) {  // steps of one source side by side: it is read once for each batch of a run
         std::stable_sort(op.begin(), op.end(), [&](uint32_t a, uint32_t b) { return source(a) < source(b); });
         for (uint32_t i : op) {
             first.push_back((uint32_t)p.ends.size());

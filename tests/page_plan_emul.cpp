@@ -47,3 +47,6 @@ extern "C" long emul_pages(size_t n, const int64_t *dst, const int64_t *src, int
         });
     return clash ? -1 : large ? -2 : reads;
 }
+
+// steps in a batch of the kernel
+extern "C" int kernel_batch() { return PAGE_BATCH; }

@@ -84,3 +84,40 @@ def test_many_moves(emul):
     emul(pages, list(range(pages)), list(range(1, pages)) + [0])
     emul(pages, rng.sample(range(pages), 3000), [rng.randint(-1, pages - 1) for _ in range(3000)])
     emul(pages, list(range(1, pages)), [0] * (pages - 1))
+
+
+# ---- at the batch of the kernel ---------------------------------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def kernel_batch(emul, tmp_path_factory):
+    so = tmp_path_factory.mktemp("page_batch") / "batch.so"
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-o", str(so), os.path.join(HERE, "page_plan_emul.cpp")])
+    return ctypes.CDLL(str(so)).kernel_batch()
+
+
+def test_reads_of_one_source_in_the_kernel(emul, kernel_batch):
+    """once for every batch that its steps take in a lane"""
+    for copies in range(1, 20):
+        assert emul(20, list(range(1, copies + 1)), [0] * copies, lanes=1, batch=kernel_batch) == -(-copies // kernel_batch)
+    assert emul(20, [5, 1, 7, 3], [2, 0, 2, 0], lanes=1, batch=kernel_batch) == 2
+
+
+@pytest.mark.parametrize("cap", [3, 4, 5, 7, 480])
+@pytest.mark.parametrize("length", [2, 3, 4, 5, 8, 9, 17, 40, 481, 1200])
+def test_cycles_in_the_kernel(emul, kernel_batch, cap, length):
+    pages = list(range(length))
+    reads = emul(length, pages, pages[1:] + pages[:1], cap=cap, batch=kernel_batch)
+    assert reads == length if length + 1 <= cap else reads > length
+
+
+@pytest.mark.parametrize("lanes", [1, 2, 7, 64])
+def test_random_moves_in_the_kernel(emul, kernel_batch, lanes):
+    rng = random.Random(lanes)
+    for _ in range(400):
+        pages = rng.randint(1, 90)
+        n = rng.randint(0, pages)
+        dst = rng.sample(range(pages), n)
+        for src in (rng.sample(dst, n), [rng.randint(-1, pages - 1) for _ in range(n)], [rng.choice([0, pages - 1]) for _ in range(n)]):
+            emul(pages, dst, src, lanes=lanes, batch=kernel_batch)
+            other = np.array([rng.randrange(1 << 40) for _ in range(pages)], dtype=np.int64)
+            emul(pages, dst, src, lanes=lanes, batch=kernel_batch, other=other)
+    emul(5000, list(range(5000)), rng.sample(range(5000), 5000), lanes=lanes, batch=kernel_batch)
