@@ -75,6 +75,81 @@ def test_positions_that_torch_negates_on_the_fly(kit):
     assert torch.equal(rot.factors(p), rot.factors(p.clone())) and not torch.equal(rot.factors(p), rot.factors(z.imag))
 
 
+# ---- what the host looks at, and what it cannot while a graph is captured ---------------------------------------------------------
+@pytest.mark.parametrize("packing", ["pairs", "interleaved"])
+def test_factors_and_plaintexts_that_are_refused(kit, packing):
+    ctx, enc, rng = kit["ctx"], kit["enc"], np.random.default_rng(2)
+    rot = ph.rotary(ctx, [1.0, 0.1], 8, 16, packing=packing)
+    x, pos = _encrypt(kit, rng, 2), torch.arange(rot.positions_per_ct, dtype=torch.float64, device="cuda")
+    good = rot.factors(pos)
+    for value in (1e9, float("nan"), complex(0, float("inf"))):
+        bad = good.clone()
+        bad[-1, 0, 5] = value
+        with pytest.raises(ValueError, match="too large"):
+            rot.encode(enc, bad, 2)
+    plain = [[enc.encode_complex_vector(ctx, v.cpu().numpy(), 2.0 ** 40, 2) for v in vec] for vec in good]
+    with pytest.raises(ValueError, match="scale mismatch"):
+        rot.apply([x], plain, kit["glk"])
+    at_prime = [[enc.encode_complex_vector(ctx, v.cpu().numpy(), float(ctx.primes[2]), 2) for v in vec] for vec in good]
+    (y,) = rot.apply([x], at_prime, kit["glk"])
+    (z,) = rot.forward(enc, [x], pos, galois_key=kit["glk"])
+    assert y.scale() == z.scale() == 2.0 ** 40 and torch.equal(y.data, z.data)  # the same coefficients, one vector after another
+    keep = torch.ones(len(pos), dtype=torch.bool, device="cuda")
+    pos[3], keep[3] = float("nan"), False
+    rot.forward(enc, [x], pos, keep=keep, galois_key=kit["glk"])
+    with pytest.raises(ValueError, match="finite"):
+        rot.forward(enc, [x], pos, galois_key=kit["glk"])
+
+
+def test_captured_rotations(kit):
+    """factors, encode and apply, and forward with positions in floating point, in one graph: nothing waits for the device"""
+    ctx, enc, rng = kit["ctx"], kit["enc"], np.random.default_rng(3)
+    rot = ph.rotary(ctx, [1.0, 0.1], 8, 16, packing="halves")
+    x, pos = _encrypt(kit, rng, 2), torch.arange(rot.positions_per_ct, dtype=torch.float64, device="cuda")
+
+    def call():
+        (y,) = rot.apply([x], rot.encode(enc, rot.factors(pos), 2), kit["glk"])
+        (z,) = rot.forward(enc, [x], pos, galois_key=kit["glk"])
+        return y.data, z.data
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y, z = call()
+    for _ in range(2):
+        pos.add_(0.5)
+        g.replay()
+        assert torch.equal(y, z) and all(torch.equal(a, y) for a in call())
+
+
+def test_resized_on_another_stream(kit):
+    """the pages that stay keep their words where the pool was made on one stream and is resized, and given back, on another"""
+    ctx = kit["ctx"]
+    cache = ph.ciphertext_cache(ctx, 1, 40, 2)
+    table = cache.allocate(20)
+    mark = torch.arange(1, 21, device="cuda")[:, None, None, None]
+    cache.data[:, :20] = mark
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for pages in (30, 25, 50, 20):
+            cache.resize(pages)
+    torch.full((2, 40, 2, 4, ctx.N), 77, dtype=torch.int64, device="cuda")  # what would take the memory given back
+    torch.cuda.current_stream().wait_stream(side)
+    assert cache.pages() == len(table) == 20 and bool((cache.data == mark).all())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cache.copy([0], [1])
+        with pytest.raises(RuntimeError, match="captured"):
+            cache.resize(30)
+    g.replay()
+    assert cache.pages() == 20 and bool((cache.data[:, 0] == 2).all())
+
+
 # ---- several queries in every arithmetic ------------------------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def pool():
