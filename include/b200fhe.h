@@ -340,7 +340,8 @@ int b2_poly_scalar(b2_ctx *ctx, int op, size_t n_limbs, const uint64_t *d_a, con
  * becomes what page src[i] was before the call, for all i at once: copies, one page into many, permutations in place. src[i] < 0:
  * a page of zeros. d_src null (or d_pool): the pool itself; else another one, [planes][src_pages][2][src_limbs][N] with
  * src_limbs >= limbs, of which the first `limbs` limbs of each polynomial are taken (mod_switch_to). dst and src are HOST arrays
- * of n, read at the call; destinations are distinct. No scratch; each thread owns the same 32 bytes of every page. */
+ * of n, read at the call; destinations are distinct. No scratch; each thread owns the same 32 bytes of every page. One launch for up
+ * to 480 steps (one a move, one more a cycle), beyond that several in the stream's order. */
 int b2_pages_move(b2_ctx *ctx, size_t limbs, size_t planes, uint64_t *d_pool, size_t pages, const uint64_t *d_src,
                   size_t src_limbs, size_t src_pages, size_t n, const int64_t *dst, const int64_t *src, void *stream);
 /* b2_multiply_sum: for every query g, the three polynomials of sum_t a[g * terms + t] x b[t] (b2_tensor_mul, summed), so that one
@@ -350,7 +351,7 @@ int b2_pages_move(b2_ctx *ctx, size_t limbs, size_t planes, uint64_t *d_pool, si
 int b2_multiply_sum(b2_ctx *ctx, size_t size_Ql, size_t queries, size_t terms, const uint64_t *const *d_a, size_t a_limbs,
                     const uint64_t *const *d_b, size_t b_limbs, uint64_t *d_out, void *stream);
 /* b2_multiply_plain_sum: out[i] = sum_t ct[i * terms + t] times pt[i * terms + t] (multiply_plain and add, src/evaluate.cu:1150-1200)
- * for n ciphertexts in one launch, 1 to 4 terms; HOST arrays of n * terms device pointers to [2][size_Ql][N] and [size_Ql][N];
+ * for n ciphertexts, 32 to a launch, 1 to 4 terms; HOST arrays of n * terms device pointers to [2][size_Ql][N] and [size_Ql][N];
  * d_out [n][2][size_Ql][N], apart from the operands. */
 int b2_multiply_plain_sum(b2_ctx *ctx, size_t size_Ql, size_t n, size_t terms, const uint64_t *const *d_ct,
                           const uint64_t *const *d_pt, uint64_t *d_out, void *stream);

@@ -66,15 +66,17 @@ void launch_pages_move(const PageArgs &a, const PageStep *steps, const uint32_t 
 // out[g] = (sum_t a0 b0, sum_t a0 b1 + a1 b0, sum_t a1 b1) mod every prime: products of the pages with the scores that weigh them,
 // summed before any of them is relinearised. A thread owns one position of a limb and walks the terms, U of them loaded before the
 // first is multiplied; sums stay in registers as the prime's arithmetic likes them (sums.cuh) and are reduced once at the end.
-// G queries share one read of the pages.
+// G queries share one read of the pages, on primes of 2^50 and more two of them.
 // Bound by HBM: 2 (G + 1) limbs a term for 3 G products. One word a thread and load keeps the sums of all arithmetics in 80 registers
-// (G = 1; 768 threads an SM with sixteen loads each in flight): 32 terms at N = 2^16, 16 limbs of 40 bits take 160.6 us (1.10 GB, 6.84
-// TB/s), 17 terms of 6 limbs at 2^14 11.3 (8.6 out of L2), with two words a thread 168 to 193. More queries take 128 registers and as many
-// terms at a time as those hold: two (24 pages at 2^15, 12 limbs, 0.47 GB) 76.6 us with five terms, 77.4 with four, 80.5 with three;
-// three (0.63 GB) 99.8 with four, 117 with three; four (0.79 GB) 126.8 with three, 129.3 with two. Four queries are where the power cap
-// is felt: after two seconds of them 136.7 us (141.3 with four products a term in place of three). Sums of three and four queries are
-// FP64 products: in 21-bit pieces, 72 registers of sums for four, 181 us; on integer primes, whose sums of 30-bit pieces are as wide, the
-// queries go two by two over the same pages (55 bits: four 182 us; 187 to 259 at once). Terms dealt to four groups of threads that join
+// (G = 1; 768 threads an SM with sixteen loads each in flight): 32 terms at N = 2^16, 16 limbs of 40 bits take 161 to 165 us (1.10 GB, 6.7 to
+// 6.8 TB/s), 17 terms of 6 limbs at 2^14 10 to 11 (some of it out of L2), with two words a thread 168 to 193. More queries take 128
+// registers. How many terms they load at a time was chosen at one length, 24 pages of 12 limbs at 2^15, in one run: two queries (0.47 GB)
+// 76.6 us with five terms (which spill 24 bytes), 77.4 with four, 80.5 with three; three (0.63 GB) 99.8 with four, 117 with three; four
+// (0.79 GB) 126.8 with three, 129.3 with two; other runs have 78.5, 101.6 and 129.1. Four queries are where the power cap is felt: after
+// two seconds of them 136.7 us (141.3 with four products a term in place of three). Sums of three and four queries are FP64 products: in
+// 21-bit pieces, 72 registers of sums for four, 181 us; on integer primes, whose sums of 30-bit pieces are as wide, the queries go two by
+// two over the same pages (55 bits: three 143 us, four 182 to 185; 187 to 259 at once). Two queries on 42 to 50 bits take 86.0 us, on 55
+// bits 94.3. Terms dealt to four groups of threads that join
 // in shared memory gain 1.3 us of 10 at 60 terms and 96 CTAs and lose everywhere else: not built.
 constexpr int SUM_T = 128;
 
@@ -215,7 +217,9 @@ void launch_multiply_sum(const SumArgs &a, uint32_t queries, cudaStream_t s) {
 
 // ---- sums of ciphertexts times plaintexts ---------------------------------------------------------------------------------
 // out[z] = sum_t ct[z][t] (.) pt[z][t], t below 4: what a rotated ciphertext is (x C + rot(x, s) A + rot(x, -s) B), for a batch of
-// them in one launch. Bound by HBM: 3 limbs a term and 2.
+// them in one launch. 3 limbs a term and 2 to read and write. Sixteen of three terms at 2^16, 16 limbs of 40 bits (1.48 GB) take 276 us,
+// 5.3 TB/s; at 2^15, 12 limbs (0.55 GB) 107, on 55 bits 94 (5.9 TB/s, a copy has 6.46). Bound by what is in flight: 92 registers leave
+// five CTAs an SM, each of which loads all its words, then multiplies, then stores.
 template <class S>
 __device__ __forceinline__ void plain_sum_body(const PlainSumArgs &a, const Mod &md) {
     const typename S::K k = S::make(md);

@@ -573,9 +573,9 @@ def multiply(ctx, a, b):
 
 def multiply_sum(ctx, a, b):
     """sum_t a[t] x b[t] of two lists of two-polynomial ciphertexts, as one three-polynomial ciphertext at the lower of the two
-    lists' levels: the tensor products of `multiply`, summed in one launch, so that one `relinearize` (and one rescale) serves all
-    of them. Where a is a list of lists (several weightings of the same b), each gives a result and b is read for up to four of them
-    at a time. No counterpart in the reference, which relinearises every product (src/attention.cu:60-90)."""
+    lists' levels: the tensor products of `multiply`, summed in one launch (64 terms a launch), so that one `relinearize` (and one
+    rescale) serves all of them. Where a is a list of lists (several weightings of the same b), each gives a result and b is read for up to
+    four of them at a time, on primes of 2^50 and more for two. No counterpart in the reference, which relinearises every product (src/attention.cu:60-90)."""
     if not len(b):
         raise ValueError("encrypteds cannot be empty")
     first, table, held = _operands(ctx, [b])

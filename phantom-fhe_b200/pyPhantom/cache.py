@@ -3,8 +3,8 @@ ciphertexts are lists kept by its application, and whose attention products, src
 
 A page is one two-polynomial ciphertext whose slots hold `positions` token positions (slots // d_total, the layout of
 `compute_qkt`); a sequence is a list of page numbers, its table. One cache holds the pages of one level in `planes` planes (K and V
-of every layer, say): a page number names the same page of every plane, and whatever is done to pages is done to all planes in one
-launch. The memory is one tensor data[planes][pages][2][limbs][N].
+of every layer, say): a page number names the same page of every plane, and whatever is done to pages is done to all planes at once:
+in one launch up to 480 steps (one a page, one more a cycle), in several, one after another, beyond that. The memory is one tensor data[planes][pages][2][limbs][N].
 
 Forked sequences share their full pages, which are counted; a page held more than once is not written to. A cache serves one
 stream at a time; calls work on torch's current stream of the context's device. Page numbers are read at the call: a captured graph
@@ -143,7 +143,7 @@ class ciphertext_cache:
 
     def fork(self, table, copies=1, tail=1):
         """`copies` new tables with the contents of `table`: all pages but the last `tail` are shared, those are copied (the last
-        page still takes positions), every plane and every copy in one launch"""
+        page still takes positions), every plane and every copy at once"""
         table, copies, tail = self._live(table), int(copies), int(tail)
         if copies < 1 or tail < 0:
             raise ValueError("ciphertext_cache: at least one copy and no negative tail are wanted")
@@ -177,7 +177,7 @@ class ciphertext_cache:
 
     def compact(self, tables):
         """Moves all allocated pages to the front of the pool, those of `tables` first and in their order (a table's pages then
-        lie one after another), in place and in one launch. Returns the tables with their new numbers; every other table that is
+        lie one after another), in place and at once. Returns the tables with their new numbers; every other table that is
         still held is out of date unless it is given too: pages outside `tables` keep their order behind them."""
         tables = [self._live(t) for t in tables]
         order = list(dict.fromkeys(p for t in tables for p in t))
