@@ -23,7 +23,7 @@ from ._native import LIB, check, current_stream as _stream, on_device
 
 _PACKINGS = {"pairs": 0, "halves": 1, "interleaved": 2}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
-CHUNK = 16  # ciphertexts that go through each kernel together
+CHUNK = 16  # ciphertexts whose encodings, products and rescales go together; rotations take them one after another
 
 
 class rotary:
@@ -38,7 +38,8 @@ class rotary:
             raise ValueError("rotary: heads * d_head must be in [1, slots]")
         if pairs < 1 or pairs > (d_head if packing == "pairs" else d_head // 2):
             raise ValueError("rotary: more pairs than a head holds")
-        if not (math.isfinite(scaling) and bool(torch.isfinite(f * 2.0 ** 64).all())):  # the angle of any integer position
+        angles = f.tolist()
+        if not (math.isfinite(scaling) and all(math.isfinite(v * 2.0 ** 64) for v in angles)):  # the angle of any integer position
             raise ValueError("rotary: the angles per position and the scaling must be finite (below 2^960)")
         a = [0] * pairs if axes is None else [int(v) for v in axes]
         if len(a) != pairs or min(a) < 0:
@@ -48,8 +49,8 @@ class rotary:
         self.positions_per_ct = context.N // 2 // (heads * d_head)
         self.inv_freq, self.axes = f, torch.tensor(a, dtype=torch.int32, device=context.device)
         steepest = {}  # the largest angle per position on each axis that a pair follows
-        for axis, angle in zip(a, f.abs().tolist()):
-            steepest[axis] = max(steepest.get(axis, 0.0), angle)
+        for axis, angle in zip(a, angles):
+            steepest[axis] = max(steepest.get(axis, 0.0), abs(angle))
         self._followed, self._steepest = torch.tensor(list(steepest), device=f.device), torch.tensor(list(steepest.values()), dtype=torch.float64, device=f.device)
         self.step = pairs if packing == "halves" else 1
         self._vecs = 1 if packing == "pairs" else 3
